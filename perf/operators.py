@@ -1,6 +1,7 @@
 """Operators of MoE layers whose weights are 8-bit floating point (e4m3) with
 one scale per 128 x 128 block, over activation rows in the same 8 bits with one
-F32 scale per 128 values: the RMSNorm that takes the residual in and writes such
+bf16 scale per 128 values (a scale needs range, not digits: the codes are
+rounded against the scale as it is stored): the RMSNorm that takes the residual in and writes such
 rows, the dense product, the two products grouped by expert over ragged
 segments (gate/up with SwiGLU, down), and the weighted sum of the experts' rows.
 
@@ -95,11 +96,11 @@ def spread_row(s, cols):
 
 def quantize(y):
     """Rows in 8 bits: (codes, scales), a scale being the largest magnitude of
-    its 128 values over 448."""
+    its 128 values over 448, rounded to bf16."""
     rows, n = y.shape
     p = torch.nn.functional.pad(y, (0, blocks(n) * BLOCK - n)).view(rows, blocks(n), BLOCK)
-    s = (p.abs().amax(2) / TOP).clamp(min=LEAST)
-    return (y / spread_row(s, n)).to(torch.float8_e4m3fn), s
+    s = (p.abs().amax(2) / TOP).clamp(min=LEAST).to(torch.bfloat16)
+    return (y / spread_row(s.float(), n)).to(torch.float8_e4m3fn), s
 
 
 def weights(gen, experts, out, n_in, stype):
@@ -199,7 +200,7 @@ def plain_norm(s):
 
 def plain_linear(s):
     w = s["w8"].float() * spread(s["ws"].float(), s["out"], s["in"])
-    x = s["x8"].float() * spread_row(s["xs"], s["in"])
+    x = s["x8"].float() * spread_row(s["xs"].float(), s["in"])
     return (x @ w.T).to(TYPES[s["y"]])
 
 
@@ -223,7 +224,7 @@ def of_experts(s, codes, scales):
 
 def plain_up(s):
     at, place, row = padded(s)
-    x = s["x8"].float() * spread_row(s["xs"], s["h"])
+    x = s["x8"].float() * spread_row(s["xs"].float(), s["h"])
     x = x[s["perm"].long()[at] // s["K"]]
     g = torch.bmm(x, of_experts(s, s["g8"], s["gs"]).transpose(1, 2).contiguous())
     u = torch.bmm(x, of_experts(s, s["u8"], s["us"]).transpose(1, 2).contiguous())
@@ -233,7 +234,7 @@ def plain_up(s):
 
 def plain_down(s):
     at, place, row = padded(s)
-    x = (s["x8"].float() * spread_row(s["xs"], s["ff"]))[at]
+    x = (s["x8"].float() * spread_row(s["xs"].float(), s["ff"]))[at]
     y = torch.bmm(x, of_experts(s, s["w8"], s["ws"]).transpose(1, 2).contiguous())
     out = torch.empty(s["perm"].numel(), s["h"], dtype=TYPES[s["y"]], device="cuda")
     out[s["perm"].long()] = y[place, row].to(out.dtype)
@@ -333,11 +334,11 @@ class Bound:
         return MoeRegionC(t.data_ptr(), t.numel() * t.element_size())
 
     def rows(self, codes, scales):
-        return self.hb.Rows8(self.region(codes), self.buffer(scales), codes.shape[0], codes.shape[1])
+        return self.hb.Rows8(self.region(codes), self.region(scales), codes.shape[0], codes.shape[1])
 
     def rows_out(self, rows, n):
         codes = torch.empty(rows, n, dtype=torch.float8_e4m3fn, device="cuda")
-        scales = torch.empty(rows, blocks(n), device="cuda")
+        scales = torch.empty(rows, blocks(n), dtype=torch.bfloat16, device="cuda")
         return codes, scales, self.rows(codes, scales)
 
     def weight(self, t, scales, dims, kind):
@@ -398,7 +399,7 @@ def used_experts(c):
 
 def work(case):
     def rows8(rows, n):
-        return rows * (n + 4 * blocks(n))
+        return rows * (n + 2 * blocks(n))
 
     kind = case["kind"]
     if kind == "norm":
@@ -423,8 +424,8 @@ def work(case):
 
 
 def exact(case, seed):
-    """The outputs in 64 bits from the definition, the codes before they are
-    rounded to 8."""
+    """The outputs in 64 bits from the definition, codes and scales before they
+    are rounded."""
     s = prepare(case, seed)
     f64 = torch.float64
 
