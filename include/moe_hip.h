@@ -45,6 +45,9 @@ typedef enum {
 
 /* DType ids (crates/model-format/src/dtype.rs:5-15). */
 enum { MOE_F32 = 0, MOE_F16 = 1, MOE_BF16 = 30 };
+/* 8-bit floating point weights (4 exponent and 3 mantissa bits, no infinities),
+ * for the *_q8 operators only; not one of the reference's ids. */
+enum { MOE_E4M3 = 256 };
 
 /* Gpu (crates/metal-backend/src/apple.rs:125-164): one device, one stream,
  * and the registry of allocations it owns. */
@@ -303,6 +306,70 @@ moe_status moe_block(moe_gpu *gpu, const moe_block_weights *w, moe_buffer x, moe
 #define MOE_NOALLOC_SCRATCH_BYTES (64ull << 20)
 moe_status moe_block_noalloc(moe_gpu *gpu, const moe_block_weights *w, moe_buffer x, moe_buffer out,
                              uint64_t tokens, const moe_block_io *io);
+
+/* ------------------------------------------ 8-bit floating point MoE -- */
+
+/* Operators for checkpoints whose weights are e4m3 with one scale per
+ * 128 x 128 block (no counterpart in the reference).  Together, over T tokens:
+ *   moe_norm_q8            residual add, RMSNorm, 8-bit rows (and F32 rows for
+ *                          the router: moe_matmul, moe_route_tokens, moe_dispatch)
+ *   moe_expert_swiglu_q8   gate/up products and SwiGLU per expert segment
+ *   moe_expert_matmul_q8   down products, back in (token, k) order
+ *   moe_mix_tokens         weighted sum over k (+ residual)
+ * and moe_matmul_q8 for dense projections.  (A shared expert is
+ * moe_expert_swiglu_q8 with E = 1, offsets {0, T} and no perm, then
+ * moe_matmul_q8.)
+ *
+ * A weight (moe_weight): dtype MOE_E4M3, bits 0, `data` the codes
+ * [E][out][in], group_size 128, `scales` one scale_type value (F32, F16 or
+ * BF16) per block, [E][ceil(out/128)][ceil(in/128)], biases unused; a value is
+ * code * scale.  dims[0] is a multiple of 16 and the codes start 16-byte
+ * aligned.
+ *
+ * Products multiply the codes exactly.  F32 outputs are F32 sums.  Outputs in
+ * BF16 or 8 bits use matrix instructions on the codes themselves, which align
+ * eight products at a time to the largest of them and cut each at 2^-13 of its
+ * power of two; sums of eight, blocks and scales join in F32. */
+
+/* Rows in 8 bits: codes [rows, n], n a multiple of 16, 16-byte aligned, and one
+ * BF16 scale per row and 128 columns, [rows, ceil(n/128)].  Quantised here:
+ * scale = bf16(max(max|v| / 448, 2^-126)), code = e4m3(v / scale), each to
+ * nearest even.  128 columns that hold an infinity or a NaN read back as NaN. */
+typedef struct {
+    moe_region codes;
+    moe_region scales;
+    uint64_t rows;
+    uint64_t n;
+} moe_rows8;
+
+/* s = x + residual (residual empty: s = x); v = s / sqrt(mean(s^2) + eps) * w
+ * over rows of q.n values; q = v in 8 bits.  Optional outputs: `sum` = s (may
+ * be exactly x or residual) and `y` = v, F32.  w: dense [n] of F32, F16 or
+ * BF16.  The RMSNorm and residual of moe_norm and moe_add. */
+moe_status moe_norm_q8(moe_gpu *gpu, moe_buffer x, moe_buffer residual, const moe_weight *w,
+                       moe_buffer sum, moe_buffer y, moe_rows8 q, float eps);
+/* y[t, o] = sum_i x[t, i] * W[o, i], W dims [in, out]; y F32 or, with y_type
+ * MOE_BF16, bf16 (two per element; an even number of values). */
+moe_status moe_matmul_q8(moe_gpu *gpu, const moe_weight *w, moe_rows8 x, moe_buffer y,
+                         uint32_t y_type);
+/* Grouped by expert, over segments as moe_dispatch writes them: position p of
+ * [offsets[e], offsets[e+1]) belongs to expert e, and perm[p] is its pair
+ * t*k + i.  q[p] = silu(x_t . G_e) * (x_t . U_e) in 8 bits, in position order;
+ * q.rows = x.rows * k positions.  perm empty: position p reads row p (k = 1).
+ * Ends past q.rows count as q.rows; positions of no segment, and positions
+ * whose perm names no row, are left as they were. */
+moe_status moe_expert_swiglu_q8(moe_gpu *gpu, const moe_weight *gate, const moe_weight *up,
+                                moe_rows8 x, moe_buffer offsets, moe_buffer perm, uint64_t k,
+                                moe_rows8 q);
+/* The same segments: y[perm[p]] = W_e x[p], one row of W's dims[1] values per
+ * pair (perm empty: y[p]); x.rows positions. */
+moe_status moe_expert_matmul_q8(moe_gpu *gpu, const moe_weight *w, moe_rows8 x,
+                                moe_buffer offsets, moe_buffer perm, moe_buffer y, uint32_t y_type);
+/* moe_mix for every token: y[t] = sum_i w[t*k + i] * x[t*k + i] (i ascending)
+ * (+ residual[t], which may be exactly y); w holds tokens * k values, x F32 or
+ * bf16 rows of y.len / tokens values. */
+moe_status moe_mix_tokens(moe_gpu *gpu, moe_buffer x, uint32_t x_type, moe_buffer w,
+                          moe_buffer residual, moe_buffer y, uint64_t tokens);
 
 /* ------------------------------------------------------ measurement -- */
 

@@ -259,6 +259,33 @@ hipError_t launch_split_rows(Prof *p, hipStream_t s, const char *name, const WDe
 hipError_t launch_tile_schedule(Prof *p, hipStream_t s, const uint32_t *offsets, uint32_t experts,
                                 uint32_t tm, uint32_t *tiles, uint32_t *ntiles);
 
+// ---- 8-bit floating point operators (k_q8_rows.hip, k_q8_mm.hip) ----
+// e4m3 codes [E][out][in], scales [E][ceil(out/128)][ceil(in/128)] of `stype`
+struct Q8Weight {
+    const uint8_t *codes;
+    const void *scales;
+    uint32_t stype, in, out, experts;
+};
+// e4m3 codes [rows, n], bf16 scales [rows, ceil(n/128)]
+struct Q8Rows {
+    uint8_t *codes;
+    uint16_t *scales;
+    uint32_t rows, n;
+};
+// (resid, sum, y: optional)
+hipError_t launch_norm_q8(Prof *p, hipStream_t s, const float *x, const float *resid, const void *w, uint32_t wtype,
+                          float *sum, float *y, uint8_t *codes, uint16_t *scales, uint32_t rows, uint32_t n,
+                          float eps);
+hipError_t launch_mix_tokens(Prof *p, hipStream_t s, const void *x, bool bf16, const float *w, const float *resid,
+                             float *y, uint32_t tokens, uint32_t k, uint32_t h);
+// y[perm[p]] = W_e x[p] over the segments of `offsets` (null: one expert, all
+// rows); perm null: y[p]
+hipError_t launch_q8_rows(Prof *p, hipStream_t s, const char *name, const Q8Weight &w, const Q8Rows &x,
+                          const uint32_t *offsets, const uint32_t *perm, void *y, bool bf16);
+// out[p] = silu(x_t . G_e) * (x_t . U_e), t = perm[p] / k (perm null: p)
+hipError_t launch_q8_swiglu(Prof *p, hipStream_t s, const Q8Weight &gate, const Q8Weight &up, const Q8Rows &x,
+                            const uint32_t *offsets, const uint32_t *perm, uint32_t k, const Q8Rows &out);
+
 // ---- fused single-token decode (k_decode.hip) ----
 struct DecodeArgs {
     WDesc router, gate, up, down, sg, su, sd, sgi;

@@ -23,6 +23,7 @@ PKG_DIR = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.path.join(PKG_DIR, "libmoe_hip.so")
 
 F32, F16, BF16 = 0, 1, 30  # crates/model-format/src/dtype.rs:5-15
+E4M3 = 256  # 8-bit floating point weights of the *_q8 operators (not one of the reference's ids)
 PATH_AUTO, PATH_OPS, PATH_GROUPED, PATH_MFMA = 0, 1, 2, 3
 
 
@@ -80,6 +81,10 @@ class MoeWeightC(C.Structure):
 
 class MoePackedWeightC(C.Structure):
     _fields_ = [("data", MoeRegionC), ("scales", MoeRegionC), ("biases", MoeRegionC)]
+
+
+class MoeRows8C(C.Structure):
+    _fields_ = [("codes", MoeRegionC), ("scales", MoeRegionC), ("rows", C.c_uint64), ("n", C.c_uint64)]
 
 
 class MoeBlockWeightsC(C.Structure):
@@ -164,6 +169,12 @@ SIGNATURES = {
     "moe_block_workspace_layout": (I32, [C.POINTER(MoeBlockWeightsC), U64, C.POINTER(MoeBlockLayoutC)]),
     "moe_block": (I32, [P, C.POINTER(MoeBlockWeightsC), BUF, BUF, U64, C.POINTER(MoeBlockIOC)]),
     "moe_block_noalloc": (I32, [P, C.POINTER(MoeBlockWeightsC), BUF, BUF, U64, C.POINTER(MoeBlockIOC)]),
+    "moe_norm_q8": (I32, [P, BUF, BUF, C.POINTER(MoeWeightC), BUF, BUF, MoeRows8C, F]),
+    "moe_matmul_q8": (I32, [P, C.POINTER(MoeWeightC), MoeRows8C, BUF, U32]),
+    "moe_expert_swiglu_q8": (I32, [P, C.POINTER(MoeWeightC), C.POINTER(MoeWeightC), MoeRows8C, BUF, BUF, U64,
+                                   MoeRows8C]),
+    "moe_expert_matmul_q8": (I32, [P, C.POINTER(MoeWeightC), MoeRows8C, BUF, BUF, BUF, U32]),
+    "moe_mix_tokens": (I32, [P, BUF, U32, BUF, BUF, BUF, U64]),
     "moe_profile_enable": (I32, [P, I32]),
     "moe_profile_count": (I32, [P, C.POINTER(U32)]),
     "moe_profile_get": (I32, [P, U32, C.c_char_p, C.c_size_t, C.POINTER(U64),
@@ -229,6 +240,13 @@ class Tensor:
         return cls(dims, np.ascontiguousarray(packed, np.uint32), bits=bits, group_size=group_size,
                    scale_type=scale_type, scales=scales, biases=biases)
 
+    @classmethod
+    def block8(cls, dims, codes, scales, scale_type=F32):
+        """8-bit floating point weight: e4m3 codes [E, out, in] and one scale per
+        128 x 128 block, [E, ceil(out/128), ceil(in/128)] (raw bits for F16/BF16)."""
+        return cls(dims, np.ascontiguousarray(codes, np.uint8), dtype=E4M3, group_size=128, scale_type=scale_type,
+                   scales=np.ascontiguousarray(scales, np.float32 if scale_type == F32 else np.uint16))
+
     def elements(self):
         return int(np.prod(self.dims))
 
@@ -277,6 +295,16 @@ class Weight:
         for i in range(3):
             c.dims[i] = dims[i] if i < len(dims) else 0
         return Weight(c, self.regions, dims, self.bits)
+
+
+class Rows8:
+    """Rows in 8 bits (moe_rows8; no reference counterpart): e4m3 codes
+    [rows, n] and one bf16 scale per row and 128 columns, as regions."""
+
+    def __init__(self, codes, scales, rows, n, buffers=()):
+        self.c = MoeRows8C(codes, scales, rows, n)
+        self.rows, self.n = rows, n
+        self.buffers = tuple(buffers)
 
 
 class PackedWeight:
@@ -446,11 +474,39 @@ class Gpu:
             c.group_size = t.group_size
         else:
             c.dtype = t.dtype
+            if t.dtype == E4M3:
+                c.scales = self._region(t.scales)
+                regions += [c.scales]
+                c.scale_type = t.scale_type
+                c.group_size = t.group_size
         c.bits = t.bits
         c.ndims = len(t.dims)
         for i, d in enumerate(t.dims):
             c.dims[i] = d
         return Weight(c, regions, t.dims, t.bits)
+
+    def rows8(self, rows, n, codes=None, scales=None):
+        """8-bit rows [rows, n]: zeros, or the given e4m3 codes (bytes) and bf16
+        scale bits.  write_rows8 and read_rows8 move their contents."""
+        nb = rows * n, rows * (-(-n // 128)) * 2
+        bufs = [self.zeros(-(-b // 4)) for b in nb]
+        r = Rows8(MoeRegionC(bufs[0].c.ptr, nb[0]), MoeRegionC(bufs[1].c.ptr, nb[1]), rows, n, bufs)
+        if codes is not None:
+            self.write_rows8(r, codes, scales)
+        return r
+
+    def write_rows8(self, r, codes, scales):
+        for b, a, dt in zip(r.buffers, (codes, scales), (np.uint8, np.uint16)):
+            raw = np.zeros(4 * len(b), np.uint8)
+            a = np.ascontiguousarray(a, dt).ravel().view(np.uint8)
+            raw[:a.size] = a
+            self.write(b, raw.view(np.float32))
+
+    def read_rows8(self, r):
+        """(codes uint8 [rows, n], bf16 scale bits uint16 [rows, ceil(n/128)])"""
+        c, s = (self.read(b).view(np.uint8) for b in r.buffers)
+        nb = -(-r.n // 128)
+        return c[:r.rows * r.n].reshape(r.rows, r.n), s.view(np.uint16)[:r.rows * nb].reshape(r.rows, nb)
 
     def pack_weight(self, weight):
         """Allocate and fill the packed copy of `weight` (one batch); None
@@ -619,6 +675,25 @@ class Batch:
     def dispatch(self, ids, tokens, k, experts, counts, offsets, perm, pos):
         self._ck(_lib.moe_dispatch(self.gpu._h, ids.c, tokens, k, experts, counts.c, offsets.c,
                                    perm.c, pos.c))
+
+    # 8-bit floating point operators (no reference counterpart)
+    def norm_q8(self, x, residual, w, sum, y, q, eps):
+        """q = RMSNorm(x + residual) * w in 8 bits; residual, sum (x + residual)
+        and y (the norm in F32) may be None."""
+        self._ck(_lib.moe_norm_q8(self.gpu._h, x.c, _c(residual), C.byref(w.c), _c(sum), _c(y), q.c, eps))
+
+    def matmul_q8(self, w, x, y, y_type=F32):
+        self._ck(_lib.moe_matmul_q8(self.gpu._h, C.byref(w.c), x.c, y.c, y_type))
+
+    def expert_swiglu_q8(self, gate, up, x, offsets, perm, k, q):
+        self._ck(_lib.moe_expert_swiglu_q8(self.gpu._h, C.byref(gate.c), C.byref(up.c), x.c, offsets.c, _c(perm), k,
+                                           q.c))
+
+    def expert_matmul_q8(self, w, x, offsets, perm, y, y_type=F32):
+        self._ck(_lib.moe_expert_matmul_q8(self.gpu._h, C.byref(w.c), x.c, offsets.c, _c(perm), y.c, y_type))
+
+    def mix_tokens(self, x, w, residual, y, tokens, x_type=F32):
+        self._ck(_lib.moe_mix_tokens(self.gpu._h, x.c, x_type, w.c, _c(residual), y.c, tokens))
 
     def copy(self, src, dst):
         self._ck(_lib.moe_copy(self.gpu._h, src.c, dst.c))

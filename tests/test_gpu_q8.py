@@ -1,0 +1,586 @@
+"""The 8-bit floating point operators on the GPU, through the public entry
+points, against their 64-bit forms (helpers_q8)."""
+import numpy as np
+import pytest
+
+from helpers_q8 import (U, Weight8, bf16, check_quantized, cut_bound, decode, encode, f32_bound, nblocks, product,
+                        quantize_rows, random_rows, rows_value, silu, spread)
+from hip_backend import BF16, E4M3, F16, F32, Batch, Buffer, GpuError, Rows8, ShapeError, Tensor
+from hip_backend.api import MoeBufferC, MoeRegionC
+from hip_backend.synth import f32_to_bf16_bits
+
+pytestmark = pytest.mark.gpu
+
+
+class Owned:
+    """Allocations of one test, released at its end."""
+
+    def __init__(self, gpu):
+        self.gpu, self.bufs = gpu, []
+
+    def upload(self, a):
+        b = self.gpu.upload(np.asarray(a))
+        self.bufs.append(b)
+        return b
+
+    def u32(self, a):
+        b = self.gpu.upload_u32(np.asarray(a))
+        self.bufs.append(b)
+        return b
+
+    def zeros(self, n, fill=None):
+        b = self.gpu.zeros(n)
+        self.bufs.append(b)
+        if fill is not None:
+            self.gpu.write(b, np.full(n, fill, np.uint32).view(np.float32))
+        return b
+
+    def rows8(self, rows, n, codes=None, scales=None):
+        r = self.gpu.rows8(rows, n, codes, scales)
+        self.bufs += r.buffers
+        return r
+
+    def weight(self, t):
+        w = self.gpu.weight_tensor(t)
+        self.bufs += [Buffer(self.gpu, MoeBufferC(), r.ptr) for r in w.regions]
+        return w
+
+    def release(self):
+        for b in self.bufs:
+            self.gpu.release(b)
+
+
+@pytest.fixture
+def own(gpu):
+    o = Owned(gpu)
+    yield o
+    o.release()
+
+
+def read_bf16(gpu, b):
+    return bf16(gpu.read_u32(b).view(np.uint16)).astype(np.float64)
+
+
+# ------------------------------------------------------------------- norm --
+def norm64(x, w, eps):
+    x = x.astype(np.float64)
+    return x / np.sqrt((x * x).mean(1, keepdims=True) + eps) * w
+
+
+NORM_SIZES = [(1, 16), (1, 2048), (3, 128), (2, 144), (5, 1360), (7, 2064), (2, 4096), (3, 6160), (2, 9232)]
+
+
+@pytest.mark.parametrize("rows,n", NORM_SIZES)
+@pytest.mark.parametrize("wtype", [F32, F16, BF16])
+def test_norm_q8(gpu, own, rows, n, wtype):
+    rng = np.random.default_rng(rows * 10000 + n)
+    x = (rng.standard_normal((rows, n)) * 3).astype(np.float32)
+    r = rng.standard_normal((rows, n)).astype(np.float32)
+    w = (1 + 0.3 * rng.standard_normal(n)).astype(np.float32)
+    if wtype == F16:
+        raw = w.astype(np.float16)
+        w64, t = raw.astype(np.float64), Tensor.dense([n], raw.view(np.uint16), F16)
+    elif wtype == BF16:
+        raw = f32_to_bf16_bits(w)
+        w64, t = bf16(raw).astype(np.float64), Tensor.dense([n], raw, BF16)
+    else:
+        w64, t = w.astype(np.float64), Tensor.dense([n], w)
+    wd, xb, rb = own.weight(t), own.upload(x), own.upload(r)
+    for resid, with_sum, with_y in [(True, True, True), (False, False, True), (True, False, False),
+                                    (False, True, False)]:
+        q, s, y = own.rows8(rows, n), own.zeros(rows * n), own.zeros(rows * n)
+        with gpu.batch() as b:
+            b.norm_q8(xb, rb if resid else None, wd, s if with_sum else None, y if with_y else None, q, 1e-6)
+        sum_ = x + r if resid else x
+        if with_sum:
+            assert np.array_equal(gpu.read(s).reshape(rows, n), sum_)
+        want = norm64(sum_, w64, 1e-6)
+        # the mean of n squares in sums of at most 64 roundings, its root and
+        # reciprocal, and two products
+        dy = (64 + 6) * U * np.abs(want)
+        codes, bits = gpu.read_rows8(q)
+        if with_y:
+            got = gpu.read(y).reshape(rows, n)
+            assert np.all(np.abs(got - want) <= dy)
+            # the scale is that of the F32 values written beside the codes
+            assert np.array_equal(bits, quantize_rows(got)[1])
+        check_quantized(codes, bits, want, dy)
+
+
+def test_norm_q8_in_place(gpu, own):
+    rng = np.random.default_rng(5)
+    rows, n = 3, 6160
+    x = rng.standard_normal((rows, n)).astype(np.float32)
+    r = rng.standard_normal((rows, n)).astype(np.float32)
+    wd = own.weight(Tensor.dense([n], np.ones(n, np.float32)))
+    out = []
+    for where in ("own", "x", "residual"):
+        xb, rb, q = own.upload(x), own.upload(r), own.rows8(rows, n)
+        s = {"own": own.zeros(rows * n), "x": xb, "residual": rb}[where]
+        with gpu.batch() as b:
+            b.norm_q8(xb, rb, wd, s, None, q, 1e-5)
+        assert np.array_equal(gpu.read(s).reshape(rows, n), x + r)
+        out.append(gpu.read_rows8(q))
+    for c, s in out[1:]:
+        assert np.array_equal(c, out[0][0]) and np.array_equal(s, out[0][1])
+
+
+def test_norm_q8_from_unaligned_buffers(gpu, own):
+    """F32 arrays that start at any element."""
+    rng = np.random.default_rng(6)
+    rows, n = 2, 400
+    x = rng.standard_normal(rows * n + 3).astype(np.float32)
+    wd = own.weight(Tensor.dense([n], np.ones(n, np.float32)))
+    xb, y, s = own.upload(x), own.zeros(rows * n + 1), own.zeros(rows * n + 2)
+    q = own.rows8(rows, n)
+    with gpu.batch() as b:
+        b.norm_q8(xb.view(3, rows * n), None, wd, s.view(2, rows * n), y.view(1, rows * n), q, 1e-6)
+    want = norm64(x[3:].reshape(rows, n), np.ones(n), 1e-6)
+    assert np.all(np.abs(gpu.read(y)[1:].reshape(rows, n) - want) <= 70 * U * np.abs(want))
+    assert np.array_equal(gpu.read(s)[2:], x[3:]) and gpu.read(y)[0] == 0
+    check_quantized(*gpu.read_rows8(q), want, 70 * U * np.abs(want))
+
+
+def test_norm_q8_of_zeros_tiny_and_non_finite_rows(gpu, own):
+    rows, n = 5, 272
+    rng = np.random.default_rng(7)
+    x = rng.standard_normal((rows, n)).astype(np.float32)
+    x[0] = 0
+    x[1, :128] = 0
+    w = np.ones(n, np.float32)
+    w[256:] = 1e-38                     # values below 448 * 2^-126
+    x[2, 3], x[3, 200] = np.inf, np.nan
+    wd, xb, q = own.weight(Tensor.dense([n], w)), own.upload(x), own.rows8(rows, n)
+    with gpu.batch() as b:
+        b.norm_q8(xb, None, wd, None, None, q, 1e-6)
+    codes, bits = gpu.read_rows8(q)
+    least = f32_to_bf16_bits(np.array([2.0 ** -126], np.float32))[0]
+    assert np.all(codes[0] & 0x7F == 0) and np.all(bits[0] == least)
+    assert np.all(codes[1, :128] & 0x7F == 0) and bits[1, 0] == least and bits[1, 1] != least and bits[1, 2] == least
+    v = rows_value(codes, bits)
+    assert np.isnan(v[3]).all()                        # NaN in the sum of squares
+    assert np.isnan(v[2, :128]).all()                  # inf * 0
+    want = norm64(x[4:], w.astype(np.float64), 1e-6)
+    check_quantized(codes[4:], bits[4:], want, 70 * U * np.abs(want) + 2.0 ** -149)
+
+
+# ------------------------------------------------------------------ dense --
+def check_rows(got, want, mag, groups, n_in, bf):
+    if bf:
+        # the output's rounding: half a bf16 step, 2^-8 of the value
+        lim = cut_bound(n_in, mag, groups)
+        lim = lim + 2.0 ** -8 * (np.abs(want) + lim)
+    else:
+        lim = f32_bound(n_in, mag)
+    bad = ~(np.abs(got - want) <= lim)
+    assert not bad.any(), (int(bad.sum()), np.argwhere(bad)[:4].tolist(),
+                           float(np.max(np.abs(got - want) / np.maximum(lim, 1e-300))))
+
+
+MATMUL_SIZES = [(1, 128, 64), (1, 16, 1), (2, 48, 15), (1, 2048, 512), (15, 144, 130), (16, 256, 256), (17, 272, 258),
+                (33, 640, 300), (64, 128, 1000), (100, 1040, 512), (129, 256, 64), (300, 384, 770)]
+
+
+@pytest.mark.parametrize("T,n_in,out", MATMUL_SIZES)
+@pytest.mark.parametrize("y_type", [F32, BF16])
+def test_matmul_q8(gpu, own, T, n_in, out, y_type):
+    if y_type == BF16 and T * out % 2:
+        pytest.skip("bf16 outputs come two to an element")
+    rng = np.random.default_rng(T * 1000 + n_in + out)
+    st = [F32, BF16, F16][(T + out) % 3]
+    w = Weight8(rng, 1, out, n_in, st)
+    codes, bits = random_rows(rng, T, n_in)
+    wd, x = own.weight(w.tensor(dense=True)), own.rows8(T, n_in, codes, bits)
+    elems = T * out if y_type == F32 else T * out // 2
+    y = own.zeros(elems + 4, 0x7F7F7F7F)
+    with gpu.batch() as b:
+        b.matmul_q8(wd, x, y.view(0, elems), y_type)
+    want, mag, g = product(rows_value(codes, bits), w.value())
+    got = gpu.read(y.view(0, elems)) if y_type == F32 else read_bf16(gpu, y.view(0, elems))
+    check_rows(got.reshape(T, out), want, mag, g, n_in, y_type == BF16)
+    assert np.all(gpu.read_u32(y)[elems:] == 0x7F7F7F7F)   # nothing past the output
+
+
+@pytest.mark.parametrize("y_type", [F32, BF16])
+@pytest.mark.parametrize("T", [1, 40, 200])
+def test_matmul_q8_every_code(gpu, own, T, y_type):
+    """One-hot rows read each code of a weight back exactly, at every column."""
+    rng = np.random.default_rng(11)
+    n_in, out = 256, 256
+    w = Weight8(rng, 1, out, n_in)
+    w.codes[0, :, :] = (np.arange(out)[:, None] + np.arange(n_in)[None, :]) % 256
+    w.codes[0, 4:][(w.codes[0, 4:] & 0x7F) == 0x7F] = 0x30   # NaN in the first four rows only
+    w.scales[:], w.bits[:] = 1, 1
+    wd = own.weight(w.tensor(dense=True))
+    cols = (np.arange(T) * 37) % n_in
+    codes = np.zeros((T, n_in), np.uint8)
+    codes[np.arange(T), cols] = encode(1.0)
+    x = own.rows8(T, n_in, codes, np.full((T, 2), 0x3F80, np.uint16))
+    y = own.zeros(T * out if y_type == F32 else T * out // 2)
+    with gpu.batch() as b:
+        b.matmul_q8(wd, x, y, y_type)
+    got = (gpu.read(y) if y_type == F32 else read_bf16(gpu, y)).reshape(T, out)
+    v = decode(w.codes[0])
+    nan = np.isnan(v).any(1)            # a NaN of the row reaches every token (NaN * 0)
+    assert nan.sum() == 4 and np.isnan(got[:, nan]).all()
+    assert np.array_equal(got[:, ~nan], v[:, cols].T[:, ~nan])
+
+
+def test_matmul_q8_wide_scales(gpu, own):
+    """Scales and values over their whole range; a NaN or infinite scale."""
+    rng = np.random.default_rng(12)
+    T, n_in, out = 20, 512, 384
+    w = Weight8(rng, 1, out, n_in)
+    w.bits[:] = (2.0 ** rng.integers(-60, 20, w.bits.shape)).astype(np.float32)
+    w.scales[:] = w.bits
+    codes, _ = random_rows(rng, T, n_in)
+    bits = f32_to_bf16_bits((2.0 ** rng.integers(-40, 40, (T, 4))).astype(np.float32)).reshape(T, 4)
+    bits[3, 1], bits[4, 2] = 0x7FC0, 0x7F80
+    wd, x, y = own.weight(w.tensor(dense=True)), own.rows8(T, n_in, codes, bits), own.zeros(T * out)
+    with gpu.batch() as b:
+        b.matmul_q8(wd, x, y)
+    got = gpu.read(y).reshape(T, out).astype(np.float64)
+    assert np.isnan(got[3]).all() and not np.isfinite(got[4]).any()
+    keep = [t for t in range(T) if t not in (3, 4)]
+    want, mag, g = product(rows_value(codes, bits)[keep], w.value())
+    check_rows(got[keep], want, mag, g, n_in, False)
+
+
+# ---------------------------------------------------------------- experts --
+def segments(rng, lens, shuffle=True):
+    """offsets and perm of segments of these lengths (pairs in a random order
+    across segments, ascending within one, as a dispatch gives them)."""
+    P = int(sum(lens))
+    offsets = np.concatenate([[0], np.cumsum(lens)]).astype(np.uint32)
+    perm = rng.permutation(P) if shuffle else np.arange(P)
+    for a, b in zip(offsets[:-1], offsets[1:]):
+        perm[a:b] = np.sort(perm[a:b])
+    return offsets, perm.astype(np.uint32)
+
+
+LENS = [
+    [1], [0, 1, 0], [2, 0, 0, 16, 1, 15, 17], [33, 0, 64, 5, 1], [100, 31, 0, 129],
+    [0] * 300 + [3] + [0] * 800 + [1, 2],        # more experts than threads, nearly all empty
+    [260, 4],
+]
+
+
+@pytest.mark.parametrize("lens", LENS, ids=lambda v: f"{len(v)}x{sum(v)}")
+@pytest.mark.parametrize("n_in,out", [(128, 64), (48, 300), (272, 130)])
+@pytest.mark.parametrize("y_type", [F32, BF16])
+def test_expert_matmul_q8(gpu, own, lens, n_in, out, y_type):
+    rng = np.random.default_rng(sum(lens) + n_in)
+    E, P = len(lens), sum(lens)
+    w = Weight8(rng, E, out, n_in, [F32, BF16, F16][P % 3])
+    codes, bits = random_rows(rng, P, n_in)
+    offsets, perm = segments(rng, lens)
+    wd, x = own.weight(w.tensor()), own.rows8(P, n_in, codes, bits)
+    ob, pb = own.u32(offsets), own.u32(perm)
+    v = rows_value(codes, bits)
+    want, mag, g = (np.zeros((P, out)) for _ in range(3))
+    for e in range(E):
+        a, b_ = offsets[e], offsets[e + 1]
+        if b_ > a:
+            want[a:b_], mag[a:b_], g[a:b_] = product(v[a:b_], w.value(e))
+    elems = P * out if y_type == F32 else P * out // 2
+    for p in (pb, None):
+        y = own.zeros(elems)
+        with gpu.batch() as b:
+            b.expert_matmul_q8(wd, x, ob, p, y, y_type)
+        got = (gpu.read(y) if y_type == F32 else read_bf16(gpu, y)).reshape(P, out)
+        if p is not None:
+            got = got[perm]
+        check_rows(got, want, mag, g, n_in, y_type == BF16)
+
+
+def swiglu64(x, gate, up, e):
+    """The SwiGLU of expert e in 64 bits and how far 8-bit sums may be off:
+    |silu'| <= 1.1, and eight roundings of the exponential, division and products."""
+    n_in = x.shape[1]
+    g, gm, gg = product(x, gate.value(e))
+    u, um, ug = product(x, up.value(e))
+    dg, du = cut_bound(n_in, gm, gg), cut_bound(n_in, um, ug)
+    a = silu(g) * u
+    return a, 1.1 * dg * (np.abs(u) + du) + np.abs(silu(g)) * du + 8 * U * np.abs(a)
+
+
+@pytest.mark.parametrize("lens", LENS, ids=lambda v: f"{len(v)}x{sum(v)}")
+@pytest.mark.parametrize("n_in,ff", [(128, 64), (48, 272), (272, 16), (256, 128)])
+def test_expert_swiglu_q8(gpu, own, lens, n_in, ff):
+    rng = np.random.default_rng(sum(lens) * 3 + n_in)
+    E, P = len(lens), sum(lens)
+    st = [F32, BF16, F16][(P + ff // 16) % 3]
+    gate, up = Weight8(rng, E, ff, n_in, st), Weight8(rng, E, ff, n_in, st)
+    offsets, perm = segments(rng, lens)
+    gd, ud, ob, pb = own.weight(gate.tensor()), own.weight(up.tensor()), own.u32(offsets), own.u32(perm)
+    for K in [k for k in (1, 2, 3) if P % k == 0]:
+        T = P // K
+        codes, bits = random_rows(rng, T, n_in)
+        x, q = own.rows8(T, n_in, codes, bits), own.rows8(P, ff)
+        with gpu.batch() as b:
+            b.expert_swiglu_q8(gd, ud, x, ob, pb, K, q)
+        v = rows_value(codes, bits)[perm // K]
+        want, dw = np.zeros((P, ff)), np.zeros((P, ff))
+        for e in range(E):
+            a, b_ = offsets[e], offsets[e + 1]
+            if b_ > a:
+                want[a:b_], dw[a:b_] = swiglu64(v[a:b_], gate, up, e)
+        check_quantized(*gpu.read_rows8(q), want, dw)
+    # no perm: position p reads row p
+    codes, bits = random_rows(rng, P, n_in)
+    x, q, q2 = own.rows8(P, n_in, codes, bits), own.rows8(P, ff), own.rows8(P, ff)
+    ident = own.u32(np.arange(P))
+    with gpu.batch() as b:
+        b.expert_swiglu_q8(gd, ud, x, ob, None, 1, q)
+        b.expert_swiglu_q8(gd, ud, x, ob, ident, 1, q2)
+    for i, j in zip(gpu.read_rows8(q), gpu.read_rows8(q2)):
+        assert np.array_equal(i, j)
+
+
+def test_expert_products_leave_other_rows(gpu, own):
+    """Positions behind the last segment, and positions whose perm names no
+    row, keep what they held; ends past the positions count as their number."""
+    rng = np.random.default_rng(21)
+    n_in, ff, E, P = 128, 48, 3, 40
+    gate, up, down = (Weight8(rng, E, ff, n_in) for _ in range(3))
+    gd, ud, dd = (own.weight(w.tensor()) for w in (gate, up, down))
+    codes, bits = random_rows(rng, P, n_in)
+    x = own.rows8(P, n_in, codes, bits)
+    perm = rng.permutation(P).astype(np.uint32)
+    for offsets, live in [([0, 5, 5, 30], np.arange(30)), ([0, 7, 20, 1000], np.arange(40)),
+                          ([3, 9, 2, 12], np.r_[3:9, 2:12]), ([50, 60, 70, 4000000000], np.arange(0))]:
+        p2 = perm.copy()
+        p2[8], p2[11] = 40, 0xFFFFFFFF
+        ob, pb = own.u32(np.array(offsets, np.uint32)), own.u32(p2)
+        q, y = own.rows8(P, ff, np.full((P, ff), 0x55, np.uint8), np.full((P, 1), 0x1234, np.uint16)), own.zeros(P * ff, 0x55555555)
+        with gpu.batch() as b:
+            b.expert_swiglu_q8(gd, ud, x, ob, pb, 1, q)
+            b.expert_matmul_q8(dd, x, ob, pb, y)
+        written = np.zeros(P, bool)
+        written[live] = True
+        written[[8, 11]] = False
+        c, s = gpu.read_rows8(q)
+        assert np.all(c[~written] == 0x55) and np.all(s[~written] == 0x1234)
+        assert not np.any(s[written] == 0x1234)
+        rows = gpu.read_u32(y).reshape(P, ff)
+        to = np.zeros(P, bool)
+        to[p2[written]] = True
+        assert np.all(rows[~to] == 0x55555555) and not np.any((rows[to] == 0x55555555).all(1))
+
+
+# -------------------------------------------------------------------- mix --
+@pytest.mark.parametrize("T,K,h", [(1, 1, 16), (1, 10, 2048), (3, 8, 130), (5, 3, 7), (64, 10, 512), (300, 2, 1028)])
+@pytest.mark.parametrize("x_type", [F32, BF16])
+def test_mix_tokens(gpu, own, T, K, h, x_type):
+    if x_type == BF16 and T * K * h % 2:
+        pytest.skip("bf16 inputs come two to an element")
+    rng = np.random.default_rng(T + K + h)
+    x = rng.standard_normal((T, K, h)).astype(np.float32)
+    if x_type == BF16:
+        raw = f32_to_bf16_bits(x.ravel())
+        x = bf16(raw).reshape(T, K, h)
+        xb = own.upload(raw.view(np.float32))
+    else:
+        xb = own.upload(x)
+    w = rng.standard_normal((T, K)).astype(np.float32)
+    r = rng.standard_normal((T, h)).astype(np.float32)
+    wb, rb, y = own.upload(w), own.upload(r), own.zeros(T * h)
+    terms = x.astype(np.float64) * w.astype(np.float64)[..., None]
+    want, mag = terms.sum(1), np.abs(terms).sum(1)
+    with gpu.batch() as b:
+        b.mix_tokens(xb, wb, None, y, T, x_type)
+    plain = gpu.read(y).reshape(T, h)
+    assert np.all(np.abs(plain - want) <= K * U * mag)
+    with gpu.batch() as b:
+        b.mix_tokens(xb, wb, rb, y, T, x_type)
+        b.mix_tokens(xb, wb, rb, rb, T, x_type)      # the residual in place
+    got = gpu.read(y).reshape(T, h)
+    assert np.all(np.abs(got - (want + r)) <= (K + 1) * U * (mag + np.abs(r)))
+    assert np.array_equal(gpu.read(rb).reshape(T, h), got)
+
+
+def test_mix_tokens_equals_mix(gpu, own):
+    rng = np.random.default_rng(4)
+    T, K, h = 3, 5, 64
+    x, w = own.upload(rng.standard_normal(T * K * h)), own.upload(rng.standard_normal(T * K))
+    y, one = own.zeros(T * h), own.zeros(T * h)
+    with gpu.batch() as b:
+        b.mix_tokens(x, w, None, y, T)
+        for t in range(T):
+            b.mix(x.view(t * K * h, K * h), w.view(t * K, K), one.view(t * h, h))
+    a, c = gpu.read(y), gpu.read(one)
+    assert np.all(np.abs(a - c) <= 2 * K * U * 20)
+
+
+# --------------------------------------------------------------- refusals --
+def test_refusals(gpu, own):
+    rng = np.random.default_rng(9)
+    E, n_in, out, T = 3, 256, 64, 6
+    wt, gt = Weight8(rng, E, out, n_in), Weight8(rng, 1, out, n_in)
+    w3, w2 = own.weight(wt.tensor()), own.weight(gt.tensor(dense=True))
+    codes, bits = random_rows(rng, T, n_in)
+    x, y = own.rows8(T, n_in, codes, bits), own.zeros(T * out)
+    q, ob, pb = own.rows8(T, out), own.u32([0, 2, 4, 6]), own.u32(np.arange(T))
+    dense = own.weight(Tensor.dense([n_in, out], rng.standard_normal(n_in * out)))
+    norm, xf = own.weight(Tensor.dense([n_in], np.ones(n_in, np.float32))), own.upload(np.ones(T * n_in))
+    other = own.weight(Weight8(rng, E, out, n_in, BF16).tensor())
+
+    def alter(w, **kw):
+        c = type(w.c).from_buffer_copy(w.c)
+        for k, v in kw.items():
+            if k == "dims":
+                for i, d in enumerate(v):
+                    c.dims[i] = d
+            else:
+                setattr(c, k, v)
+        return type(w)(c, w.regions, w.dims, 0)
+
+    def rows(r, **kw):
+        a = {"codes": r.c.codes, "scales": r.c.scales, "rows": r.rows, "n": r.n}
+        a.update(kw)
+        return Rows8(a["codes"], a["scales"], a["rows"], a["n"])
+
+    short = MoeRegionC(x.c.codes.ptr, x.c.codes.bytes - 1)
+    odd = MoeRegionC(x.c.codes.ptr + 4, (T - 1) * n_in)
+    foreign = MoeRegionC(0x1000, x.c.codes.bytes)
+    bad = [
+        lambda b: b.matmul_q8(dense, x, y),
+        lambda b: b.matmul_q8(w3, x, y),
+        lambda b: b.matmul_q8(alter(w2, group_size=64), x, y),
+        lambda b: b.matmul_q8(alter(w2, scale_type=7), x, y),
+        lambda b: b.matmul_q8(alter(w2, dims=[n_in, out + 1]), x, y),
+        lambda b: b.matmul_q8(alter(w2, dims=[n_in // 2 - 8, 2 * out]), x, y),
+        lambda b: b.matmul_q8(alter(w2, dims=[0, out]), x, y),
+        lambda b: b.matmul_q8(w2, rows(x, n=128, rows=2 * T), y),
+        lambda b: b.matmul_q8(w2, rows(x, rows=T - 1), y),
+        lambda b: b.matmul_q8(w2, rows(x, rows=0), y),
+        lambda b: b.matmul_q8(w2, rows(x, codes=short), y),
+        lambda b: b.matmul_q8(w2, rows(x, codes=foreign), y),
+        lambda b: b.matmul_q8(w2, rows(x, codes=odd, rows=T - 1,
+                                       scales=MoeRegionC(x.c.scales.ptr, (T - 1) * 4)), y.view(0, (T - 1) * out)),
+        lambda b: b.matmul_q8(w2, x, y.view(0, T * out - 1)),
+        lambda b: b.matmul_q8(w2, x, y, BF16),
+        lambda b: b.matmul_q8(w2, x, y, F16),
+        lambda b: b.matmul_q8(w2, x, Buffer(gpu, MoeBufferC(w2.c.data.ptr, T * out), 0)),
+        lambda b: b.matmul(w2, xf, y, T),                       # the F32 op takes no 8-bit weights
+        lambda b: b.expert_matmul_q8(w2, x, ob, pb, y),
+        lambda b: b.expert_matmul_q8(w3, x, ob.view(0, 3), pb, y),
+        lambda b: b.expert_matmul_q8(w3, x, ob, pb.view(0, T - 1), y),
+        lambda b: b.expert_swiglu_q8(w3, other, x, ob, pb, 1, q),
+        lambda b: b.expert_swiglu_q8(w3, alter(w3, dims=[n_in, out - 1, E]), x, ob, pb, 1, q),
+        lambda b: b.expert_swiglu_q8(w3, w3, x, ob, pb, 2, q),
+        lambda b: b.expert_swiglu_q8(w3, w3, x, ob, pb, 0, q),
+        lambda b: b.expert_swiglu_q8(w3, w3, x, ob, None, 2, q),
+        lambda b: b.expert_swiglu_q8(w3, w3, x, ob, pb, 1, x),
+        lambda b: b.norm_q8(xf, None, w2, None, None, x, 1e-6),
+        lambda b: b.norm_q8(xf, None, norm, None, None, x, 0.0),
+        lambda b: b.norm_q8(xf, None, norm, None, None, x, float("nan")),
+        lambda b: b.norm_q8(xf, None, norm, None, xf, x, 1e-6),
+        lambda b: b.norm_q8(xf.view(0, n_in), None, norm, None, None, x, 1e-6),
+        lambda b: b.norm_q8(xf, xf.view(0, n_in), norm, None, None, x, 1e-6),
+        lambda b: b.norm_q8(xf, None, norm, y, None, x, 1e-6),
+        lambda b: b.mix_tokens(xf, y.view(0, T), None, y.view(0, T * n_in // 8), T),
+        lambda b: b.mix_tokens(xf, y.view(0, T), None, xf, T),
+        lambda b: b.mix_tokens(xf, y.view(0, T), None, y, 0),
+        lambda b: b.mix_tokens(xf, y.view(0, T + 1), None, y, T),
+        lambda b: b.mix_tokens(xf, y.view(0, T), None, y, T, F16),
+    ]
+    before = gpu.read(y).copy()
+    for i, f in enumerate(bad):
+        b = Batch(gpu)
+        try:
+            with pytest.raises(ShapeError):
+                f(b)
+                print("not refused:", i)
+        finally:
+            b.finish()
+    assert np.array_equal(gpu.read(y), before)
+    # outside of a batch
+    b = Batch(gpu, begin=False)
+    with pytest.raises(ShapeError):
+        b.matmul_q8(w2, x, y)
+
+
+# ------------------------------------------------------------------ chain --
+def chain(b, o, d):
+    """One MoE block over T tokens by the operators."""
+    b.norm_q8(d["x"], d["r"], d["norm"], d["sum"], d["xn"], d["x8"], 1e-6)
+    b.matmul(d["router"], d["xn"], d["logits"], d["T"])
+    b.route_tokens(d["logits"], d["ids"], d["w"], d["T"], True)
+    b.dispatch(d["ids"], d["T"], d["K"], d["E"], d["counts"], d["offsets"], d["perm"], d["pos"])
+    b.expert_swiglu_q8(d["gate"], d["up"], d["x8"], d["offsets"], d["perm"], d["K"], d["a8"])
+    b.expert_matmul_q8(d["down"], d["a8"], d["offsets"], d["perm"], d["y"], d["ytype"])
+    b.mix_tokens(d["y"], d["w"], d["sum"], d["out"], d["T"], d["ytype"])
+
+
+def chain_state(own, rng, T, h, E, K, ff, ytype):
+    d = {"T": T, "K": K, "E": E, "ytype": ytype}
+    d["host"] = {n: Weight8(rng, E, *s) for n, s in (("gate", (ff, h)), ("up", (ff, h)), ("down", (h, ff)))}
+    for n, w in d["host"].items():
+        d[n] = own.weight(w.tensor())
+    d["hx"], d["hr"] = (rng.standard_normal((T, h)).astype(np.float32) for _ in range(2))
+    d["x"], d["r"] = own.upload(d["hx"]), own.upload(d["hr"])
+    d["hn"] = (1 + 0.1 * rng.standard_normal(h)).astype(np.float32)
+    d["norm"] = own.weight(Tensor.dense([h], d["hn"]))
+    d["router"] = own.weight(Tensor.dense([h, E], rng.standard_normal(h * E) * 0.05))
+    for n, s in (("sum", T * h), ("xn", T * h), ("logits", T * E), ("ids", T * K), ("w", T * K), ("counts", E),
+                 ("offsets", E + 1), ("perm", T * K), ("pos", T * K), ("out", T * h),
+                 ("y", T * K * h // (2 if ytype == BF16 else 1))):
+        d[n] = own.zeros(s)
+    d["x8"], d["a8"] = own.rows8(T, h), own.rows8(T * K, ff)
+    return d
+
+
+@pytest.mark.parametrize("T,h,E,K,ff,ytype", [(1, 256, 8, 2, 128, F32), (7, 272, 5, 3, 48, F32),
+                                              (70, 256, 6, 4, 144, BF16), (200, 128, 4, 2, 256, BF16)])
+def test_chain(gpu, own, T, h, E, K, ff, ytype):
+    """The operators as a block uses them, each stage against 64 bits over what
+    the stage before it wrote; then captured and replayed over new inputs."""
+    rng = np.random.default_rng(T * 7 + h)
+    d = chain_state(own, rng, T, h, E, K, ff, ytype)
+    with gpu.batch() as b:
+        chain(b, own, d)
+
+    def check():
+        s = d["hx"] + d["hr"]
+        assert np.array_equal(gpu.read(d["sum"]).reshape(T, h), s)
+        xn = norm64(s, d["hn"].astype(np.float64), 1e-6)
+        check_quantized(*gpu.read_rows8(d["x8"]), xn, 70 * U * np.abs(xn))
+        off, perm = gpu.read_u32(d["offsets"]), gpu.read_u32(d["perm"])
+        ids, w = gpu.read_u32(d["ids"]).reshape(T, K), gpu.read(d["w"]).reshape(T, K).astype(np.float64)
+        assert off[E] == T * K
+        x = rows_value(*gpu.read_rows8(d["x8"]))
+        a8 = gpu.read_rows8(d["a8"])
+        a = rows_value(*a8)
+        want, dw = np.zeros((T * K, ff)), np.zeros((T * K, ff))
+        y, ym, yg = (np.zeros((T * K, h)) for _ in range(3))
+        for e in range(E):
+            p = np.arange(off[e], off[e + 1])
+            assert np.array_equal(ids.ravel()[perm[p]], np.full(p.size, e))
+            if p.size:
+                want[p], dw[p] = swiglu64(x[perm[p] // K], d["host"]["gate"], d["host"]["up"], e)
+                y[perm[p]], ym[perm[p]], yg[perm[p]] = product(a[p], d["host"]["down"].value(e))
+        check_quantized(*a8, want, dw)
+        got = (read_bf16(gpu, d["y"]) if ytype == BF16 else gpu.read(d["y"]).astype(np.float64)).reshape(T * K, h)
+        check_rows(got, y, ym, yg, ff, ytype == BF16)
+        terms = got.reshape(T, K, h) * w[..., None]
+        out = terms.sum(1) + s
+        assert np.all(np.abs(gpu.read(d["out"]).reshape(T, h) - out) <= (K + 1) * U * (np.abs(terms).sum(1) + np.abs(s)))
+
+    check()
+    cap = gpu.capture()
+    with cap as b:
+        chain(b, own, d)
+    for _ in range(3):
+        d["hx"] = rng.standard_normal((T, h)).astype(np.float32)
+        gpu.write(d["x"], d["hx"])
+        with gpu.batch() as b:
+            b.graph(cap.graph)
+        check()
+        first = [gpu.read(d[n]).copy() for n in ("out", "y")] + list(gpu.read_rows8(d["a8"]))
+        with gpu.batch() as b:
+            chain(b, own, d)
+        again = [gpu.read(d[n]) for n in ("out", "y")] + list(gpu.read_rows8(d["a8"]))
+        for i, j in zip(first, again):
+            assert np.array_equal(np.asarray(i).view(np.uint8), np.asarray(j).view(np.uint8))
+    cap.graph.destroy()

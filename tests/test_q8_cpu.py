@@ -1,0 +1,58 @@
+"""The 8-bit floating point operators' plain forms and host side, on the CPU."""
+import ctypes as C
+
+import numpy as np
+
+from helpers_q8 import POS, TABLE, Weight8, decode, encode, nblocks, quantize_rows, random_rows, rows_value
+from hip_backend import BF16, E4M3, F16, F32, api
+
+
+def test_e4m3_codes_round_to_nearest_even():
+    codes = np.arange(256, dtype=np.uint8)
+    real = (codes & 0x7F) != 0x7F
+    assert np.array_equal(encode(decode(codes[real])), codes[real])
+    assert POS[-1] == 448 and POS[1] == 2.0 ** -9 and np.all(np.diff(POS) > 0)
+    for a, b, even in zip(POS[:-1], POS[1:], range(126)):
+        want = even if even % 2 == 0 else even + 1
+        assert encode((a + b) / 2) == want
+        assert encode(np.nextafter((a + b) / 2, 1e9)) == even + 1
+    assert encode(464.0) == 0x7E and np.isnan(TABLE[encode(465.0)]) and np.isnan(TABLE[encode(np.nan)])
+
+
+def test_quantized_rows_read_back_within_half_a_step():
+    rng = np.random.default_rng(3)
+    y = rng.standard_normal((5, 272)).astype(np.float32)
+    y[1] = 0
+    y[2, :128] *= np.float32(1e-42)
+    codes, bits = quantize_rows(y)
+    got = rows_value(codes, bits)
+    assert np.all(np.abs(got - y)[[0, 2, 3, 4]] <= np.maximum(2.0 ** -4 * np.abs(y), 2.0 ** -10 * np.abs(y).max())[[0, 2, 3, 4]])
+    assert np.all(got[1] == 0)
+    y[3, 200] = np.inf
+    y[4, 5] = np.nan
+    codes, bits = quantize_rows(y)
+    got = rows_value(codes, bits)
+    assert np.isnan(got[3, 128:256]).all() and np.isfinite(got[3, :128]).all() and np.isfinite(got[3, 256:]).all()
+    assert np.isnan(got[4, :128]).all() and np.isfinite(got[4, 128:]).all()
+
+
+def test_entries_without_a_gpu_are_refused():
+    lib = api.load_library()
+    w, r, b = api.MoeWeightC(), api.MoeRows8C(), api.MoeBufferC()
+    assert lib.moe_norm_q8(None, b, b, C.byref(w), b, b, r, 1e-6) == 3
+    assert lib.moe_matmul_q8(None, C.byref(w), r, b, 0) == 3
+    assert lib.moe_expert_swiglu_q8(None, C.byref(w), C.byref(w), r, b, b, 1, r) == 3
+    assert lib.moe_expert_matmul_q8(None, C.byref(w), r, b, b, b, 0) == 3
+    assert lib.moe_mix_tokens(None, b, 0, b, b, b, 1) == 3
+
+
+def test_block8_tensors_hold_codes_and_block_scales():
+    rng = np.random.default_rng(1)
+    for st, size in ((F32, 4), (F16, 2), (BF16, 2)):
+        w = Weight8(rng, 3, 130, 272, st)
+        t = w.tensor()
+        assert t.dims == [272, 130, 3] and t.dtype == E4M3 and t.bits == 0 and t.group_size == 128
+        assert t.data.nbytes == 3 * 130 * 272 and t.scales.nbytes == 3 * 2 * 3 * size
+        assert w.value(2).shape == (130, 272) and nblocks(272) == 3
+    codes, bits = random_rows(rng, 4, 48)
+    assert codes.shape == (4, 48) and bits.shape == (4, 1)
