@@ -293,7 +293,7 @@ class Bound:
             self.out = torch.empty(s["tokens"], s["out"], dtype=TYPES[s["y"]], device="cuda")
             self.y, self.ytype = self.buffer(self.out), hb.F32 if s["y"] == "f32" else hb.BF16
         elif kind == "mix":
-            self.x, self.xtype = self.buffer(s["x"]), hb.F32 if s["x"] == "f32" else hb.BF16
+            self.x, self.xtype = self.buffer(s["x"]), hb.F32 if s["x"].dtype == f32 else hb.BF16
             self.w, self.r = self.buffer(s["w"]), self.maybe(s["r"])
             self.out = torch.empty(s["tokens"], s["h"], dtype=f32, device="cuda")
             self.y = self.buffer(self.out)
