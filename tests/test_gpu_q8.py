@@ -261,7 +261,7 @@ def segments(rng, lens, shuffle=True):
 LENS = [
     [1], [0, 1, 0], [2, 0, 0, 16, 1, 15, 17], [33, 0, 64, 5, 1], [100, 31, 0, 129],
     [0] * 300 + [3] + [0] * 800 + [1, 2],        # more experts than threads, nearly all empty
-    [260, 4],
+    [260, 4], [70, 96, 65, 97],
 ]
 
 
