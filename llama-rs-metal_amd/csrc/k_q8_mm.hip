@@ -63,10 +63,12 @@ struct Tile {
     uint32_t e, m0, end, ct;
 };
 constexpr uint32_t kXcds = 8;
-template <int BM>
-__device__ __forceinline__ bool find_tile(const Args &a, Tile &t, uint32_t *lds /* 8 words */) {
+constexpr int kFind = 12;  // its words of LDS
+template <int BM, int NW>
+__device__ __forceinline__ bool find_tile(const Args &a, Tile &t, uint32_t *lds) {
+    static_assert(NW + 3 <= kFind, "LDS words");
     const uint32_t tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-    const uint32_t per = (a.experts + kThreads - 1) / kThreads, e0 = tid * per;
+    const uint32_t per = (a.experts + 64 * NW - 1) / (64 * NW), e0 = tid * per;
     auto seg = [&](uint32_t e, uint32_t &lo, uint32_t &n) {
         lo = min(a.offsets[e], a.P);
         const uint32_t hi = min(a.offsets[e + 1], a.P);
@@ -89,8 +91,12 @@ __device__ __forceinline__ bool find_tile(const Args &a, Tile &t, uint32_t *lds 
         if (lane == 63) lds[wv] = incl;
         __syncthreads();
         before = incl - mine;
-        for (uint32_t v = 0; v < wv; v++) before += lds[v];
-        total = lds[0] + lds[1] + lds[2] + lds[3];
+        total = 0;
+#pragma unroll
+        for (uint32_t v = 0; v < NW; v++) {
+            if (v < wv) before += lds[v];
+            total += lds[v];
+        }
     }
     const uint64_t items = (uint64_t)total * a.col_tiles, range = (items + kXcds - 1) / kXcds;
     const uint64_t item = blockIdx.x % kXcds * range + blockIdx.x / kXcds;
@@ -106,18 +112,18 @@ __device__ __forceinline__ bool find_tile(const Args &a, Tile &t, uint32_t *lds 
             uint32_t lo, n;
             const uint32_t hi = seg(e0 + i, lo, n);
             if (tile - before < n) {
-                lds[4] = e0 + i;
-                lds[5] = lo + (tile - before) * BM;
-                lds[6] = hi;
+                lds[NW] = e0 + i;
+                lds[NW + 1] = lo + (tile - before) * BM;
+                lds[NW + 2] = hi;
                 break;
             }
             before += n;
         }
     }
     __syncthreads();
-    t.e = __builtin_amdgcn_readfirstlane(lds[4]);
-    t.m0 = __builtin_amdgcn_readfirstlane(lds[5]);
-    t.end = min(__builtin_amdgcn_readfirstlane(lds[6]), t.m0 + BM);
+    t.e = __builtin_amdgcn_readfirstlane(lds[NW]);
+    t.m0 = __builtin_amdgcn_readfirstlane(lds[NW + 1]);
+    t.end = min(__builtin_amdgcn_readfirstlane(lds[NW + 2]), t.m0 + BM);
     return true;
 }
 
@@ -163,162 +169,249 @@ __device__ __forceinline__ f32x4q block_dot(const Operand<true> &a, const Operan
     return c;
 }
 
-// The outputs of a wave's 64 weight rows (from n0) for NS token tiles: acc[j][i]
-// holds row tile j, token tile i; to[i] is where the lane's token of tile i goes.
-template <int MODE, int NS, int TT>
-__device__ __forceinline__ void store_tile(const Args &a, const f32x4q (&acc)[4][NS], const uint32_t (&to)[NS],
-                                           uint32_t n0, uint32_t ct, uint32_t wv, uint32_t *tops) {
-    constexpr int BM = 16 * TT;
-    const uint32_t lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4, ob = (a.out + 127) / 128;
-    if constexpr (MODE == SWIGLU) {
-        const uint32_t col = n0 + 8 * q;
-        const bool cols_in = col < a.out;  // (out is a multiple of 16: all eight columns or none)
-        float act[NS][8];
+// The outputs of a wave's row tiles for NS token tiles of 16: acc[j][i] holds row
+// tile j, token tile i; the lane's rows are neighbours from `col` on; to[i] is
+// where the lane's token of tile i goes.
+template <int MODE, int RT, int NS>
+__device__ __forceinline__ void store_rows(const Args &a, const f32x4q (&acc)[RT][NS], const uint32_t (&to)[NS],
+                                           uint32_t col) {
+    // whole groups of four where every row starts aligned
+    const bool vec = a.out % 4 == 0 && (reinterpret_cast<uintptr_t>(a.y) & 15u) == 0;
 #pragma unroll
-        for (int i = 0; i < NS; i++) {
-            uint32_t top = 0;
+    for (int i = 0; i < NS; i++) {
+        if (to[i] == 0xffffffffu) continue;
+        const uint64_t at = (uint64_t)to[i] * a.out + col;
 #pragma unroll
-            for (int r = 0; r < 8; r++) {
-                const float g = acc[r / 4][i][r % 4], u = acc[2 + r / 4][i][r % 4];
-                act[i][r] = g / (1.0f + expf(-g)) * u;
-                if (cols_in) top = max(top, abs_word(act[i][r]));
-            }
-            top = max_xor32_u(max_xor16_u(top));
-            if (q == 0) tops[wv * BM + 16 * i + c] = top;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < NS; i++) {
-            const uint32_t at = 16 * i + c;
-            const uint32_t sb = q8_scale_bits(max(max(tops[at], tops[BM + at]), max(tops[2 * BM + at], tops[3 * BM + at])));
-            if (to[i] == 0xffffffffu) continue;
-            const float r = 1.0f / bf16_to_f32(sb);
-            if (cols_in)
-                *reinterpret_cast<u32x2q *>(a.codes + (uint64_t)to[i] * a.out + col) =
-                    u32x2q{q8_codes4(act[i][0], act[i][1], act[i][2], act[i][3], r),
-                           q8_codes4(act[i][4], act[i][5], act[i][6], act[i][7], r)};
-            if (wv == 0 && q == 0) a.scales[(uint64_t)to[i] * ob + ct] = (uint16_t)sb;
-        }
-    } else {
-        const uint32_t col = n0 + 16 * q;
-        // whole groups of four where every row starts aligned
-        const bool vec = a.out % 4 == 0 && (reinterpret_cast<uintptr_t>(a.y) & 15u) == 0;
-#pragma unroll
-        for (int i = 0; i < NS; i++) {
-            if (to[i] == 0xffffffffu) continue;
-            const uint64_t at = (uint64_t)to[i] * a.out + col;
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const f32x4q v = acc[j][i];
-                const uint32_t cj = col + 4 * j;
-                if constexpr (MODE == F32OUT) {
-                    float *y = static_cast<float *>(a.y) + at + 4 * j;
-                    if (vec) {
-                        if (cj < a.out) *reinterpret_cast<f32x4q *>(y) = v;
-                    } else {
-#pragma unroll
-                        for (int r = 0; r < 4; r++)
-                            if (cj + r < a.out) y[r] = v[r];
-                    }
+        for (int j = 0; j < RT; j++) {
+            const f32x4q v = acc[j][i];
+            const uint32_t cj = col + 4 * j;
+            if constexpr (MODE == F32OUT) {
+                float *y = static_cast<float *>(a.y) + at + 4 * j;
+                if (vec) {
+                    if (cj < a.out) *reinterpret_cast<f32x4q *>(y) = v;
                 } else {
-                    uint16_t *y = static_cast<uint16_t *>(a.y) + at + 4 * j;
-                    uint32_t b[4];
 #pragma unroll
-                    for (int r = 0; r < 4; r++) b[r] = bf16_bits(v[r]);
-                    if (vec) {
-                        if (cj < a.out) *reinterpret_cast<u32x2q *>(y) = u32x2q{b[0] | b[1] << 16, b[2] | b[3] << 16};
-                    } else {
+                    for (int r = 0; r < 4; r++)
+                        if (cj + r < a.out) y[r] = v[r];
+                }
+            } else {
+                uint16_t *y = static_cast<uint16_t *>(a.y) + at + 4 * j;
+                uint32_t b[4];
 #pragma unroll
-                        for (int r = 0; r < 4; r++)
-                            if (cj + r < a.out) y[r] = (uint16_t)b[r];
-                    }
+                for (int r = 0; r < 4; r++) b[r] = bf16_bits(v[r]);
+                if (vec) {
+                    if (cj < a.out) *reinterpret_cast<u32x2q *>(y) = u32x2q{b[0] | b[1] << 16, b[2] | b[3] << 16};
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        if (cj + r < a.out) y[r] = (uint16_t)b[r];
                 }
             }
         }
     }
 }
 
-// TT: token tiles of 16 per block.
-template <int MODE, int TT>
-__global__ __launch_bounds__(kThreads) void mm_kernel(Args a) {
-    constexpr bool kF16 = MODE == F32OUT;
-    constexpr int BM = 16 * TT;
-    __shared__ uint32_t lds[8];
-    __shared__ uint32_t tops[MODE == SWIGLU ? kWaves * BM : 1];
-    Tile t;
-    if (!find_tile<BM>(a, t, lds)) return;
-    const uint32_t ct = t.ct;
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, c = lane & 15, q = lane >> 4;
-    // the wave's rows: SWIGLU 32 gate and 32 up rows of one run of 32 outputs
-    const uint32_t n0 = MODE == SWIGLU ? ct * (kBlockRows / 2) + wv * 32 : ct * kBlockRows + wv * kWaveRows;
-    const uint8_t *wrow[4];
+// SWIGLU: row tiles 0 .. RT/2 - 1 of acc are gate rows, the rest their up rows.
+// The waves of the block hold 128 output columns of its tokens: the largest
+// magnitude of each token goes through LDS (tops: [NW][BM]).
+template <int RT, int NS, int BM, int NW>
+__device__ __forceinline__ void store_swiglu(const Args &a, const f32x4q (&acc)[RT][NS], const uint32_t (&to)[NS],
+                                             uint32_t col, uint32_t ct, uint32_t wv, uint32_t *tops) {
+    constexpr int V = 2 * RT;  // columns a lane holds
+    const uint32_t lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4, ob = (a.out + 127) / 128;
+    const bool cols_in = col < a.out;  // (out is a multiple of 16: all of the lane's columns or none)
+    float act[NS][V];
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const uint32_t r = MODE == SWIGLU ? n0 + 8 * (c >> 2) + 4 * (j & 1) + (c & 3) : n0 + 16 * (c >> 2) + 4 * j + (c & 3);
-        const uint8_t *base = MODE == SWIGLU && j >= 2 ? a.w2 : a.w;
-        wrow[j] = base + ((uint64_t)t.e * a.out + min(r, a.out - 1)) * a.in;  // rows past `out` are not stored
+    for (int i = 0; i < NS; i++) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int r = 0; r < V; r++) {
+            const float g = acc[r / 4][i][r % 4], u = acc[RT / 2 + r / 4][i][r % 4];
+            act[i][r] = g / (1.0f + expf(-g)) * u;
+            if (cols_in) top = max(top, abs_word(act[i][r]));
+        }
+        top = max_xor32_u(max_xor16_u(top));
+        if (q == 0) tops[wv * BM + 16 * i + c] = top;
     }
-    const uint32_t ob = (a.out + 127) / 128;
-    const uint64_t srow = ((uint64_t)t.e * ob + min(n0 / 128, ob - 1)) * a.kb;
-    // the lane's tokens (positions past the segment's end repeat its first row and are not stored)
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NS; i++) {
+        const uint32_t at = 16 * i + c;
+        uint32_t top = tops[at];
+#pragma unroll
+        for (int v = 1; v < NW; v++) top = max(top, tops[v * BM + at]);
+        const uint32_t sb = q8_scale_bits(top);
+        if (to[i] == 0xffffffffu) continue;
+        const float r = 1.0f / bf16_to_f32(sb);
+        if (cols_in) {
+            uint32_t *o = reinterpret_cast<uint32_t *>(a.codes + (uint64_t)to[i] * a.out + col);
+            if constexpr (V == 8)
+                *reinterpret_cast<u32x2q *>(o) =
+                    u32x2q{q8_codes4(act[i][0], act[i][1], act[i][2], act[i][3], r),
+                           q8_codes4(act[i][4], act[i][5], act[i][6], act[i][7], r)};
+            else
+                *o = q8_codes4(act[i][0], act[i][1], act[i][2], act[i][3], r);
+        }
+        if (wv == 0 && q == 0) a.scales[(uint64_t)to[i] * ob + ct] = (uint16_t)sb;
+    }
+}
+
+// Few rows per expert: the time is the weights' way from memory, so what counts
+// is how many of their loads are in flight.  A wave owns RT row tiles (SWIGLU: 16
+// gate rows and their up rows) and a range of the blocks of 128 columns (KS waves
+// share rows; their sums join through LDS in order); the codes of D blocks are
+// loaded ahead into registers, the token rows' with them.  The scales of up to
+// kChunk blocks wait in LDS as F32, loaded before the codes so that their wait
+// leaves the codes in flight.
+constexpr uint32_t kChunk = 64;
+
+template <int MODE, int RT, int TT, int KS, int NW>
+struct StreamLds {
+    float sx[kChunk][16 * TT];
+    float sw[MODE == SWIGLU ? 2 : 1][kChunk];
+    float red[KS > 1 ? NW - NW / KS : 1][KS > 1 ? 64 * RT * TT * 4 : 1];
+    uint32_t tops[MODE == SWIGLU ? NW * 16 * TT : 1];
+    uint32_t find[kFind];
+};
+
+template <int MODE, int RT, int TT, int KS, int NW, int D>
+__global__ __launch_bounds__(64 * NW, 2) void stream_kernel(Args a) {
+    constexpr bool kF16 = MODE == F32OUT;
+    constexpr int BM = 16 * TT, RG = NW / KS;  // RG: groups of rows in the block
+    constexpr int kCols = MODE == SWIGLU ? 16 : 16 * RT;  // outputs of a wave
+    static_assert(MODE != SWIGLU || (RT == 2 && KS == 1 && NW == 8), "128 output columns a block");
+    static_assert(RG * kCols <= 128 && 128 % (RG * kCols) == 0, "a block's rows share their scales");
+    __shared__ __attribute__((aligned(16))) StreamLds<MODE, RT, TT, KS, NW> lds;
+    Tile t;
+    if (!find_tile<BM, NW>(a, t, lds.find)) return;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, c = lane & 15, q = lane >> 4;
+    const uint32_t wv = __builtin_amdgcn_readfirstlane(tid >> 6), rg = wv / KS, ks = wv % KS;
+    const uint32_t n0 = t.ct * (RG * kCols) + rg * kCols, nb = min(n0, a.out - 1);
+    const uint32_t nk = a.kb, tail = a.in % 128, ob = (a.out + 127) / 128;
+    // weights: one resource per matrix from row nb on, a lane's rows as offsets
+    // (rows past `out` repeat the last and are not stored)
+    const uint64_t wbase = ((uint64_t)t.e * a.out + nb) * a.in;
+    const uint32_t wbytes = (uint32_t)min((uint64_t)(a.out - nb) * a.in, (uint64_t)0xffffffffu);
+    const __amdgpu_buffer_rsrc_t rw = buffer_rsrc(a.w + wbase, wbytes);
+    const __amdgpu_buffer_rsrc_t rw2 = MODE == SWIGLU ? buffer_rsrc(a.w2 + wbase, wbytes) : rw;
+    uint32_t woff[RT];
+#pragma unroll
+    for (int j = 0; j < RT; j++) {
+        const uint32_t r = MODE == SWIGLU ? n0 + c : n0 + 4 * RT * (c >> 2) + 4 * j + (c & 3);
+        woff[j] = (min(r, a.out - 1) - nb) * a.in + 16 * q;
+    }
+    // positions past the tile's end read its first row; outputs go to to[]
+    auto source = [&](uint32_t p) -> uint32_t {
+        const uint32_t pp = p < t.end ? p : t.m0;
+        if (MODE != SWIGLU) return pp;
+        return min((a.perm ? a.perm[pp] : pp) / a.kdiv, a.xrows - 1);
+    };
     const uint8_t *xrow[TT];
-    const uint16_t *xsrow[TT];
-    uint32_t to[TT];  // where the position's outputs go: a row, or 0xffffffff for nowhere
+    uint32_t to[TT];
 #pragma unroll
     for (int i = 0; i < TT; i++) {
         const uint32_t p = t.m0 + 16 * i + c;
         const bool live = p < t.end;
-        const uint32_t pair = a.perm ? a.perm[live ? p : t.m0] : (live ? p : t.m0);
-        uint32_t row;
-        if (MODE == SWIGLU) {
-            row = pair / a.kdiv;
-            to[i] = live && row < a.xrows ? p : 0xffffffffu;
-        } else {
-            row = live ? p : t.m0;
+        const uint32_t pair = a.perm ? a.perm[live ? p : t.m0] : p;
+        if (MODE == SWIGLU)
+            to[i] = live && pair / a.kdiv < a.xrows ? p : 0xffffffffu;
+        else
             to[i] = live && pair < a.P ? pair : 0xffffffffu;
-        }
-        row = min(row, a.xrows - 1);
-        xrow[i] = a.x + (uint64_t)row * a.in;
-        xsrow[i] = a.xs + (uint64_t)row * a.kb;
+        xrow[i] = a.x + (uint64_t)source(p) * a.in + 16 * q;
     }
-    f32x4q acc[4][TT] = {};
-    for (uint32_t kb = 0; kb < a.kb; kb++) {
-        const uint32_t k = kb * 128 + 16 * q;
-        // columns past `in`: the weights' codes are zero, the tokens' any of the row
-        const bool lo_in = k < a.in, hi_in = k + 64 < a.in;
-        const uint32_t klo = lo_in ? k : 0, khi = hi_in ? k + 64 : 0;
-        Codes wc[4], xc[TT];
-        const u32x4q zero = {0, 0, 0, 0};
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            wc[j].lo = *reinterpret_cast<const u32x4q *>(wrow[j] + klo);
-            wc[j].hi = *reinterpret_cast<const u32x4q *>(wrow[j] + khi);
-            if (!lo_in) wc[j].lo = zero;
-            if (!hi_in) wc[j].hi = zero;
+    const uint64_t swrow = ((uint64_t)t.e * ob + min(n0 / 128, ob - 1)) * nk;
+    f32x4q acc[RT][TT] = {};
+    for (uint32_t k0 = 0; k0 < nk; k0 += kChunk) {
+        const uint32_t kn = min(kChunk, nk - k0);        // blocks of this chunk
+        const uint32_t len = (kn + KS - 1) / KS;         // and of the wave's range in it
+        const uint32_t kbeg = ks * len, kend = min(kbeg + len, kn);
+        if (k0) __syncthreads();                         // the last chunk's scales are read
+        for (uint32_t i = tid; i < kn * BM; i += 64 * NW)
+            lds.sx[i / BM][i % BM] = bf16_to_f32(a.xs[(uint64_t)source(t.m0 + i % BM) * nk + k0 + i / BM]);
+        if (tid < kn) {
+            lds.sw[0][tid] = scale_at(a.ws, a.stype, swrow + k0 + tid);
+            if constexpr (MODE == SWIGLU) lds.sw[1][tid] = scale_at(a.ws2, a.stype, swrow + k0 + tid);
         }
-        float sx[TT];
+        Codes w[D][RT], x[D][TT];
+        auto load = [&](int d, uint32_t kb) {  // blocks past the chunk's end: its last again, with a scale of zero
+            const uint32_t k = k0 + min(kb, kn - 1), k128 = k * 128;
+            const bool last = tail && k + 1 == nk;
+            const uint32_t lo = last && 16 * q >= tail ? 0 : 16 * q, hi = last && 16 * q + 64 >= tail ? 0 : 16 * q + 64;
 #pragma unroll
-        for (int i = 0; i < TT; i++) {
-            const uint32_t klast = kb * 128;  // (a row's codes past `in` are replaced by ones of this block)
-            xc[i].lo = *reinterpret_cast<const u32x4q *>(xrow[i] + (lo_in ? k : klast));
-            xc[i].hi = *reinterpret_cast<const u32x4q *>(xrow[i] + (hi_in ? k + 64 : klast));
-            sx[i] = bf16_to_f32(xsrow[i][kb]);
-        }
-        const float sw = scale_at(a.ws, a.stype, srow + kb);
-        const float sw2 = MODE == SWIGLU ? scale_at(a.ws2, a.stype, srow + kb) : sw;
+            for (int j = 0; j < RT; j++) {
+                const __amdgpu_buffer_rsrc_t r = MODE == SWIGLU && j == 1 ? rw2 : rw;
+                w[d][j].lo = __builtin_bit_cast(u32x4q, __builtin_amdgcn_raw_buffer_load_b128(r, woff[j], k128, 0));
+                w[d][j].hi = __builtin_bit_cast(u32x4q, __builtin_amdgcn_raw_buffer_load_b128(r, woff[j] + 64, k128, 0));
+            }
 #pragma unroll
-        for (int i = 0; i < TT; i++) {
-            const Operand<kF16> xo(xc[i]);
+            for (int i = 0; i < TT; i++) {
+                const uint8_t *row = xrow[i] - 16 * q + k128;
+                x[d][i].lo = *reinterpret_cast<const u32x4q *>(row + lo);
+                x[d][i].hi = *reinterpret_cast<const u32x4q *>(row + hi);
+            }
+        };
+        auto use = [&](int d, uint32_t kb) {
+            const uint32_t kc = min(kb, kn - 1);
+            const bool live = kb < kend;
+            if (tail && k0 + kc + 1 == nk) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const f32x4q d = block_dot(Operand<kF16>(wc[j]), xo);
-                const float s = sx[i] * (MODE == SWIGLU && j >= 2 ? sw2 : sw);
+                for (int j = 0; j < RT; j++) {
+                    if (16 * q >= tail) w[d][j].lo = u32x4q{0, 0, 0, 0};
+                    if (16 * q + 64 >= tail) w[d][j].hi = u32x4q{0, 0, 0, 0};
+                }
+            }
+            const float sw = live ? lds.sw[0][kc] : 0.f;
+            const float sw2 = MODE == SWIGLU ? (live ? lds.sw[MODE == SWIGLU][kc] : 0.f) : sw;
 #pragma unroll
-                for (int r = 0; r < 4; r++) acc[j][i][r] = fmaf(d[r], s, acc[j][i][r]);
+            for (int i = 0; i < TT; i++) {
+                const Operand<kF16> xo(x[d][i]);
+                const float sx = live ? lds.sx[kc][16 * i + c] : 0.f;
+#pragma unroll
+                for (int j = 0; j < RT; j++) {
+                    const f32x4q p = block_dot(Operand<kF16>(w[d][j]), xo);
+                    const float s = sx * (MODE == SWIGLU && j == 1 ? sw2 : sw);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[j][i][e] = fmaf(p[e], s, acc[j][i][e]);
+                }
+            }
+        };
+#pragma unroll
+        for (int d = 0; d < D; d++) load(d, kbeg + d);
+        __syncthreads();
+        uint32_t kb = kbeg;
+        for (; kb + D < kend; kb += D) {
+#pragma unroll
+            for (int d = 0; d < D; d++) {
+                use(d, kb + d);
+                load(d, kb + D + d);
             }
         }
+#pragma unroll
+        for (int d = 0; d < D; d++) use(d, kb + d);
     }
-    store_tile<MODE, TT, TT>(a, acc, to, n0, ct, wv, tops);
+    if constexpr (KS > 1) {
+        if (ks > 0) {
+            float *r = lds.red[rg * (KS - 1) + ks - 1];
+#pragma unroll
+            for (int j = 0; j < RT; j++)
+#pragma unroll
+                for (int i = 0; i < TT; i++)
+                    *reinterpret_cast<f32x4q *>(r + ((j * TT + i) * 64 + lane) * 4) = acc[j][i];
+        }
+        __syncthreads();
+        if (ks > 0) return;
+#pragma unroll
+        for (int v = 0; v < KS - 1; v++)
+#pragma unroll
+            for (int j = 0; j < RT; j++)
+#pragma unroll
+                for (int i = 0; i < TT; i++)
+                    acc[j][i] += *reinterpret_cast<const f32x4q *>(lds.red[rg * (KS - 1) + v] + ((j * TT + i) * 64 + lane) * 4);
+    }
+    if constexpr (MODE == SWIGLU)
+        store_swiglu<RT, TT, BM, NW>(a, acc, to, n0 + 4 * q, t.ct, wv, lds.tops);
+    else
+        store_rows<MODE, RT, TT>(a, acc, to, n0 + 4 * RT * q);
 }
 
 // The same product for many rows per expert: a block of 128 (64 for F32 outputs)
@@ -337,7 +430,7 @@ struct TileLds {
     float sx[2][kGroup][BM];
     float sw[2][2][kGroup];
     uint32_t tops[kWaves * BM];
-    uint32_t find[8];
+    uint32_t find[kFind];
 };
 
 template <int MODE, int TT, int NS>
@@ -468,14 +561,17 @@ __device__ __forceinline__ void tile_body(const Args &a, const Tile &t, TileLds<
 #pragma unroll
         for (int j = 0; j < 4; j++) w[j] = wn[j];
     }
-    store_tile<MODE, NS, TT>(a, acc, to, n0, t.ct, wv, lds.tops);
+    if constexpr (MODE == SWIGLU)
+        store_swiglu<4, NS, BM, kWaves>(a, acc, to, n0 + 8 * q, t.ct, wv, lds.tops);
+    else
+        store_rows<MODE, 4, NS>(a, acc, to, n0 + 16 * q);
 }
 
 template <int MODE, int TT>
 __global__ __launch_bounds__(kThreads, 2) void tile_kernel(Args a) {
     __shared__ __attribute__((aligned(16))) TileLds<16 * TT> lds;
     Tile t;
-    if (!find_tile<16 * TT>(a, t, lds.find)) return;
+    if (!find_tile<16 * TT, kWaves>(a, t, lds.find)) return;
     // token tiles in use, in steps of a quarter (32 rows of 128)
     const uint32_t live = t.end - t.m0;
     if constexpr (TT == 8) {
@@ -491,26 +587,48 @@ __global__ __launch_bounds__(kThreads, 2) void tile_kernel(Args a) {
 
 }  // namespace q8
 
-static hipError_t launch_q8(Prof *p, hipStream_t s, const char *name, int mode, q8::Args a) {
-    const uint32_t per_block = mode == q8::SWIGLU ? q8::kBlockRows / 2 : q8::kBlockRows;
-    a.col_tiles = (a.out + per_block - 1) / per_block;
+// The stream kernel's forms of one mode: its outputs per block and its kernel.
+struct Form {
+    uint32_t cols, threads;
+    void (*kernel)(q8::Args);
+};
+template <int MODE, int TT>
+static Form stream_form(uint32_t out, uint32_t kb, uint64_t tiles) {
+    using namespace q8;
+    if constexpr (MODE == SWIGLU) {
+        return Form{128, 512, stream_kernel<SWIGLU, 2, TT, 1, 8, TT == 1 ? 4 : 3>};
+    } else {
+        // waves of 16 rows, split along the columns until the launch has 1024 of
+        // them or each two blocks; 32 rows where there are plenty
+        const uint64_t waves = (uint64_t)((out + 15) / 16) * tiles;
+        if (waves >= 4096) return Form{128, 256, stream_kernel<MODE, 2, TT, 1, 4, TT == 1 ? 4 : 3>};
+        if (waves >= 1024 || kb < 4) return Form{64, 256, stream_kernel<MODE, 1, TT, 1, 4, TT == 1 ? 8 : 4>};
+        if (waves >= 512 || kb < 8) return Form{32, 256, stream_kernel<MODE, 1, TT, 2, 4, 4>};
+        if (waves >= 256 || kb < 16) return Form{16, 256, stream_kernel<MODE, 1, TT, 4, 4, 4>};
+        return Form{16, 512, stream_kernel<MODE, 1, TT, 8, 8, 4>};
+    }
+}
+template <int MODE>
+static hipError_t launch_q8(Prof *p, hipStream_t s, const char *name, q8::Args a) {
+    using namespace q8;
     a.kb = (a.in + 127) / 128;
     const uint32_t experts = a.offsets ? a.experts : 1;
-    // DMA offsets are 32-bit
-    const bool tiled = a.P > 16ull * experts && (uint64_t)a.xrows * a.in < 0xffffffffull;
-    const uint32_t bm = !tiled ? 16 : mode == q8::F32OUT ? 64 : 128;
     // every non-empty segment may end in a partial tile
-    const uint64_t tiles = a.P / bm + (a.offsets ? (experts < a.P ? experts : a.P) : (a.P % bm != 0));
-    const uint64_t blocks = (tiles * a.col_tiles + q8::kXcds - 1) / q8::kXcds * q8::kXcds;
+    auto max_tiles = [&](uint32_t bm) {
+        return a.P / bm + (a.offsets ? (uint64_t)(experts < a.P ? experts : a.P) : (uint64_t)(a.P % bm != 0));
+    };
+    // DMA offsets are 32-bit
+    const bool tiled = a.P > 32ull * experts && (uint64_t)a.xrows * a.in < 0xffffffffull;
+    const bool two = a.P > 8ull * experts;
+    const uint32_t bm = tiled ? (MODE == F32OUT ? 64 : 128) : two && !(experts == 1 && a.P <= 16) ? 32 : 16;
+    const uint64_t tiles = max_tiles(bm);
+    const Form f = tiled      ? Form{MODE == SWIGLU ? 128u : 256u, 256, tile_kernel<MODE, MODE == F32OUT ? 4 : 8>}
+                   : bm == 32 ? stream_form<MODE, 2>(a.out, a.kb, tiles)
+                              : stream_form<MODE, 1>(a.out, a.kb, tiles);
+    a.col_tiles = (a.out + f.cols - 1) / f.cols;
+    const uint64_t blocks = (tiles * a.col_tiles + kXcds - 1) / kXcds * kXcds;
     if (blocks > 0x7fffffffull) return hipErrorInvalidConfiguration;
-    using namespace q8;
-    auto kern = tiled ? (mode == SWIGLU   ? tile_kernel<SWIGLU, 8>
-                         : mode == F32OUT ? tile_kernel<F32OUT, 4>
-                                          : tile_kernel<BF16OUT, 8>)
-                      : (mode == SWIGLU   ? mm_kernel<SWIGLU, 1>
-                         : mode == F32OUT ? mm_kernel<F32OUT, 1>
-                                          : mm_kernel<BF16OUT, 1>);
-    return launch_kernel(p, name, kern, dim3((uint32_t)blocks), dim3(kThreads), 0, s, a);
+    return launch_kernel(p, name, f.kernel, dim3((uint32_t)blocks), dim3(f.threads), 0, s, a);
 }
 
 hipError_t launch_q8_rows(Prof *p, hipStream_t s, const char *name, const Q8Weight &w, const Q8Rows &x,
@@ -519,7 +637,7 @@ hipError_t launch_q8_rows(Prof *p, hipStream_t s, const char *name, const Q8Weig
     a.w = w.codes, a.ws = w.scales, a.stype = w.stype, a.in = w.in, a.out = w.out, a.experts = w.experts;
     a.x = x.codes, a.xs = x.scales, a.xrows = x.rows, a.P = x.rows;
     a.offsets = offsets, a.perm = perm, a.y = y, a.kdiv = 1;
-    return launch_q8(p, s, name, bf16 ? q8::BF16OUT : q8::F32OUT, a);
+    return bf16 ? launch_q8<q8::BF16OUT>(p, s, name, a) : launch_q8<q8::F32OUT>(p, s, name, a);
 }
 
 hipError_t launch_q8_swiglu(Prof *p, hipStream_t s, const Q8Weight &gate, const Q8Weight &up, const Q8Rows &x,
@@ -530,7 +648,7 @@ hipError_t launch_q8_swiglu(Prof *p, hipStream_t s, const Q8Weight &gate, const 
     a.x = x.codes, a.xs = x.scales, a.xrows = x.rows, a.P = out.rows;
     a.offsets = offsets, a.perm = perm, a.kdiv = k;
     a.codes = out.codes, a.scales = out.scales;
-    return launch_q8(p, s, "expert_swiglu_q8", q8::SWIGLU, a);
+    return launch_q8<q8::SWIGLU>(p, s, "expert_swiglu_q8", a);
 }
 
 }  // namespace moehip
