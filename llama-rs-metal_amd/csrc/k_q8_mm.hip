@@ -274,8 +274,8 @@ struct StreamLds {
     uint32_t find[kFind];
 };
 
-template <int MODE, int RT, int TT, int KS, int NW, int D>
-__global__ __launch_bounds__(64 * NW, 2) void stream_kernel(Args a) {
+template <int MODE, int RT, int TT, int KS, int NW, int D, int WPS>
+__global__ __launch_bounds__(64 * NW, WPS) void stream_kernel(Args a) {
     constexpr bool kF16 = MODE == F32OUT;
     constexpr int BM = 16 * TT, RG = NW / KS;  // RG: groups of rows in the block
     constexpr int kCols = MODE == SWIGLU ? 16 : 16 * RT;  // outputs of a wave
@@ -596,16 +596,16 @@ template <int MODE, int TT>
 static Form stream_form(uint32_t out, uint32_t kb, uint64_t tiles) {
     using namespace q8;
     if constexpr (MODE == SWIGLU) {
-        return Form{128, 512, stream_kernel<SWIGLU, 2, TT, 1, 8, TT == 1 ? 4 : 3>};
+        return Form{128, 512, stream_kernel<SWIGLU, 2, TT, 1, 8, TT == 1 ? 2 : 3, TT == 1 ? 4 : 2>};
     } else {
         // waves of 16 rows, split along the columns until the launch has 1024 of
         // them or each two blocks; 32 rows where there are plenty
         const uint64_t waves = (uint64_t)((out + 15) / 16) * tiles;
-        if (waves >= 4096) return Form{128, 256, stream_kernel<MODE, 2, TT, 1, 4, TT == 1 ? 4 : 3>};
-        if (waves >= 1024 || kb < 4) return Form{64, 256, stream_kernel<MODE, 1, TT, 1, 4, TT == 1 ? 8 : 4>};
-        if (waves >= 512 || kb < 8) return Form{32, 256, stream_kernel<MODE, 1, TT, 2, 4, 4>};
-        if (waves >= 256 || kb < 16) return Form{16, 256, stream_kernel<MODE, 1, TT, 4, 4, 4>};
-        return Form{16, 512, stream_kernel<MODE, 1, TT, 8, 8, 4>};
+        if (waves >= 4096) return Form{128, 256, stream_kernel<MODE, 2, TT, 1, 4, TT == 1 ? 2 : 3, TT == 1 ? 4 : 2>};
+        if (waves >= 1024 || kb < 4) return Form{64, 256, stream_kernel<MODE, 1, TT, 1, 4, TT == 1 ? 8 : 4, 2>};
+        if (waves >= 512 || kb < 8) return Form{32, 256, stream_kernel<MODE, 1, TT, 2, 4, 4, 2>};
+        if (waves >= 256 || kb < 16) return Form{16, 256, stream_kernel<MODE, 1, TT, 4, 4, 4, 2>};
+        return Form{16, 512, stream_kernel<MODE, 1, TT, 8, 8, 4, 2>};
     }
 }
 template <int MODE>
