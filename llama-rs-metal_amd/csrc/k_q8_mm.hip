@@ -37,7 +37,7 @@ constexpr int kThreads = 256, kWaves = 4;
 constexpr int kWaveRows = 64;                     // weight rows per wave
 constexpr int kBlockRows = kWaveRows * kWaves;    // and per block
 
-enum { SWIGLU = 0, F32OUT = 1, BF16OUT = 2 };
+enum { SWIGLU = 0, F32OUT = 1, BF16OUT = 2, ACT = 3 };  // ACT: SwiGLU as F32 rows
 
 struct Args {
     const uint8_t *w, *w2;        // codes (w2: the up weights of SWIGLU)
@@ -211,6 +211,8 @@ __device__ __forceinline__ void store_rows(const Args &a, const f32x4q (&acc)[RT
     }
 }
 
+__device__ __forceinline__ float swiglu_of(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+
 // SWIGLU: row tiles 0 .. RT/2 - 1 of acc are gate rows, the rest their up rows.
 // The waves of the block hold 128 output columns of its tokens: the largest
 // magnitude of each token goes through LDS (tops: [NW][BM]).
@@ -227,7 +229,7 @@ __device__ __forceinline__ void store_swiglu(const Args &a, const f32x4q (&acc)[
 #pragma unroll
         for (int r = 0; r < V; r++) {
             const float g = acc[r / 4][i][r % 4], u = acc[RT / 2 + r / 4][i][r % 4];
-            act[i][r] = g / (1.0f + expf(-g)) * u;
+            act[i][r] = swiglu_of(g, u);
             if (cols_in) top = max(top, abs_word(act[i][r]));
         }
         top = max_xor32_u(max_xor16_u(top));
@@ -264,11 +266,12 @@ __device__ __forceinline__ void store_swiglu(const Args &a, const f32x4q (&acc)[
 // kChunk blocks wait in LDS as F32, loaded before the codes so that their wait
 // leaves the codes in flight.
 constexpr uint32_t kChunk = 64;
+constexpr uint64_t kSplitBlocks = 512;
 
 template <int MODE, int RT, int TT, int KS, int NW>
 struct StreamLds {
     float sx[kChunk][16 * TT];
-    float sw[MODE == SWIGLU ? 2 : 1][kChunk];
+    float sw[MODE == SWIGLU || MODE == ACT ? 2 : 1][kChunk];
     float red[KS > 1 ? NW - NW / KS : 1][KS > 1 ? 64 * RT * TT * 4 : 1];
     uint32_t tops[MODE == SWIGLU ? NW * 16 * TT : 1];
     uint32_t find[kFind];
@@ -276,10 +279,11 @@ struct StreamLds {
 
 template <int MODE, int RT, int TT, int KS, int NW, int D, int WPS>
 __global__ __launch_bounds__(64 * NW, WPS) void stream_kernel(Args a) {
-    constexpr bool kF16 = MODE == F32OUT;
+    constexpr bool kF16 = MODE == F32OUT, kGated = MODE == SWIGLU || MODE == ACT;
     constexpr int BM = 16 * TT, RG = NW / KS;  // RG: groups of rows in the block
-    constexpr int kCols = MODE == SWIGLU ? 16 : 16 * RT;  // outputs of a wave
-    static_assert(MODE != SWIGLU || (RT == 2 && KS == 1 && NW == 8), "128 output columns a block");
+    constexpr int kCols = kGated ? 16 : 16 * RT;  // outputs of a wave
+    static_assert(!kGated || RT == 2, "gate rows and their up rows");
+    static_assert(MODE != SWIGLU || (KS == 1 && NW == 8), "128 output columns a block");
     static_assert(RG * kCols <= 128 && 128 % (RG * kCols) == 0, "a block's rows share their scales");
     __shared__ __attribute__((aligned(16))) StreamLds<MODE, RT, TT, KS, NW> lds;
     Tile t;
@@ -293,17 +297,17 @@ __global__ __launch_bounds__(64 * NW, WPS) void stream_kernel(Args a) {
     const uint64_t wbase = ((uint64_t)t.e * a.out + nb) * a.in;
     const uint32_t wbytes = (uint32_t)min((uint64_t)(a.out - nb) * a.in, (uint64_t)0xffffffffu);
     const __amdgpu_buffer_rsrc_t rw = buffer_rsrc(a.w + wbase, wbytes);
-    const __amdgpu_buffer_rsrc_t rw2 = MODE == SWIGLU ? buffer_rsrc(a.w2 + wbase, wbytes) : rw;
+    const __amdgpu_buffer_rsrc_t rw2 = kGated ? buffer_rsrc(a.w2 + wbase, wbytes) : rw;
     uint32_t woff[RT];
 #pragma unroll
     for (int j = 0; j < RT; j++) {
-        const uint32_t r = MODE == SWIGLU ? n0 + c : n0 + 4 * RT * (c >> 2) + 4 * j + (c & 3);
+        const uint32_t r = kGated ? n0 + c : n0 + 4 * RT * (c >> 2) + 4 * j + (c & 3);
         woff[j] = (min(r, a.out - 1) - nb) * a.in + 16 * q;
     }
     // positions past the tile's end read its first row; outputs go to to[]
     auto source = [&](uint32_t p) -> uint32_t {
         const uint32_t pp = p < t.end ? p : t.m0;
-        if (MODE != SWIGLU) return pp;
+        if (!kGated) return pp;
         return min((a.perm ? a.perm[pp] : pp) / a.kdiv, a.xrows - 1);
     };
     const uint8_t *xrow[TT];
@@ -313,7 +317,7 @@ __global__ __launch_bounds__(64 * NW, WPS) void stream_kernel(Args a) {
         const uint32_t p = t.m0 + 16 * i + c;
         const bool live = p < t.end;
         const uint32_t pair = a.perm ? a.perm[live ? p : t.m0] : p;
-        if (MODE == SWIGLU)
+        if (kGated)
             to[i] = live && pair / a.kdiv < a.xrows ? p : 0xffffffffu;
         else
             to[i] = live && pair < a.P ? pair : 0xffffffffu;
@@ -330,7 +334,7 @@ __global__ __launch_bounds__(64 * NW, WPS) void stream_kernel(Args a) {
             lds.sx[i / BM][i % BM] = bf16_to_f32(a.xs[(uint64_t)source(t.m0 + i % BM) * nk + k0 + i / BM]);
         if (tid < kn) {
             lds.sw[0][tid] = scale_at(a.ws, a.stype, swrow + k0 + tid);
-            if constexpr (MODE == SWIGLU) lds.sw[1][tid] = scale_at(a.ws2, a.stype, swrow + k0 + tid);
+            if constexpr (kGated) lds.sw[1][tid] = scale_at(a.ws2, a.stype, swrow + k0 + tid);
         }
         Codes w[D][RT], x[D][TT];
         auto load = [&](int d, uint32_t kb) {  // blocks past the chunk's end: its last again, with a scale of zero
@@ -339,7 +343,7 @@ __global__ __launch_bounds__(64 * NW, WPS) void stream_kernel(Args a) {
             const uint32_t lo = last && 16 * q >= tail ? 0 : 16 * q, hi = last && 16 * q + 64 >= tail ? 0 : 16 * q + 64;
 #pragma unroll
             for (int j = 0; j < RT; j++) {
-                const __amdgpu_buffer_rsrc_t r = MODE == SWIGLU && j == 1 ? rw2 : rw;
+                const __amdgpu_buffer_rsrc_t r = kGated && j == 1 ? rw2 : rw;
                 w[d][j].lo = __builtin_bit_cast(u32x4q, __builtin_amdgcn_raw_buffer_load_b128(r, woff[j], k128, 0));
                 w[d][j].hi = __builtin_bit_cast(u32x4q, __builtin_amdgcn_raw_buffer_load_b128(r, woff[j] + 64, k128, 0));
             }
@@ -361,7 +365,7 @@ __global__ __launch_bounds__(64 * NW, WPS) void stream_kernel(Args a) {
                 }
             }
             const float sw = live ? lds.sw[0][kc] : 0.f;
-            const float sw2 = MODE == SWIGLU ? (live ? lds.sw[MODE == SWIGLU][kc] : 0.f) : sw;
+            const float sw2 = kGated ? (live ? lds.sw[kGated][kc] : 0.f) : sw;
 #pragma unroll
             for (int i = 0; i < TT; i++) {
                 const Operand<kF16> xo(x[d][i]);
@@ -369,7 +373,7 @@ __global__ __launch_bounds__(64 * NW, WPS) void stream_kernel(Args a) {
 #pragma unroll
                 for (int j = 0; j < RT; j++) {
                     const f32x4q p = block_dot(Operand<kF16>(w[d][j]), xo);
-                    const float s = sx * (MODE == SWIGLU && j == 1 ? sw2 : sw);
+                    const float s = sx * (kGated && j == 1 ? sw2 : sw);
 #pragma unroll
                     for (int e = 0; e < 4; e++) acc[j][i][e] = fmaf(p[e], s, acc[j][i][e]);
                 }
@@ -410,7 +414,17 @@ __global__ __launch_bounds__(64 * NW, WPS) void stream_kernel(Args a) {
     }
     if constexpr (MODE == SWIGLU)
         store_swiglu<RT, TT, BM, NW>(a, acc, to, n0 + 4 * q, t.ct, wv, lds.tops);
-    else
+    else if constexpr (MODE == ACT) {
+        if (n0 + 4 * q >= a.out) return;  // (out is a multiple of 16)
+#pragma unroll
+        for (int i = 0; i < TT; i++) {
+            if (to[i] == 0xffffffffu) continue;
+            f32x4q v;
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = swiglu_of(acc[0][i][e], acc[1][i][e]);
+            *reinterpret_cast<f32x4q *>(static_cast<float *>(a.y) + (uint64_t)to[i] * a.out + n0 + 4 * q) = v;
+        }
+    } else
         store_rows<MODE, RT, TT>(a, acc, to, n0 + 4 * RT * q);
 }
 
@@ -585,6 +599,41 @@ __global__ __launch_bounds__(kThreads, 2) void tile_kernel(Args a) {
     }
 }
 
+// F32 rows of the positions that a segment holds, in 8 bits; one block per
+// position.  16 lanes hold the 128 columns of a scale.
+__global__ __launch_bounds__(kThreads) void quantize_kernel(Args a, const float *act) {
+    __shared__ uint32_t held;
+    const uint32_t p = blockIdx.x, tid = threadIdx.x;
+    if (tid == 0) held = 0;
+    __syncthreads();
+    uint32_t mine = 0;
+    for (uint32_t e = tid; e < a.experts; e += kThreads) mine |= a.offsets[e] <= p && p < a.offsets[e + 1];
+    if (mine) held = 1;
+    const uint32_t pair = a.perm ? a.perm[p] : p, ob = (a.out + 127) / 128;
+    const bool row = pair / a.kdiv < a.xrows;
+    __syncthreads();
+    if (!held || !row) return;
+    for (uint32_t i = 8 * tid; (i & ~127u) < a.out; i += 8 * kThreads) {
+        float v[8] = {};
+        const bool live = i < a.out;  // (out is a multiple of 16)
+        const float *from = act + (uint64_t)p * a.out + i;
+        if (live) {
+            const f32x4q lo = *reinterpret_cast<const f32x4q *>(from), hi = *reinterpret_cast<const f32x4q *>(from + 4);
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = lo[j], v[4 + j] = hi[j];
+        }
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) top = max(top, abs_word(v[j]));
+        const uint32_t sb = q8_scale_bits(row16_max(top));
+        if (!live) continue;
+        const float r = 1.0f / bf16_to_f32(sb);
+        *reinterpret_cast<u32x2q *>(a.codes + (uint64_t)p * a.out + i) =
+            u32x2q{q8_codes4(v[0], v[1], v[2], v[3], r), q8_codes4(v[4], v[5], v[6], v[7], r)};
+        if ((tid & 15) == 0) a.scales[(uint64_t)p * ob + i / 128] = (uint16_t)sb;
+    }
+}
+
 }  // namespace q8
 
 // The stream kernel's forms of one mode: its outputs per block and its kernel.
@@ -592,15 +641,19 @@ struct Form {
     uint32_t cols, threads;
     void (*kernel)(q8::Args);
 };
+// Waves of 16 rows, split along the columns until the launch has 1024 of them
+// or each two blocks; 32 rows where there are plenty.
 template <int MODE, int TT>
 static Form stream_form(uint32_t out, uint32_t kb, uint64_t tiles) {
     using namespace q8;
+    const uint64_t waves = (uint64_t)((out + 15) / 16) * tiles;
     if constexpr (MODE == SWIGLU) {
         return Form{128, 512, stream_kernel<SWIGLU, 2, TT, 1, 8, TT == 1 ? 2 : 3, TT == 1 ? 4 : 2>};
+    } else if constexpr (MODE == ACT) {
+        if (waves >= 1024 || kb < 4) return Form{64, 256, stream_kernel<ACT, 2, TT, 1, 4, 4, 2>};
+        if (waves >= 512 || kb < 8) return Form{32, 256, stream_kernel<ACT, 2, TT, 2, 4, 4, 2>};
+        return Form{16, 256, stream_kernel<ACT, 2, TT, 4, 4, 4, 2>};
     } else {
-        // waves of 16 rows, split along the columns until the launch has 1024 of
-        // them or each two blocks; 32 rows where there are plenty
-        const uint64_t waves = (uint64_t)((out + 15) / 16) * tiles;
         if (waves >= 4096) return Form{128, 256, stream_kernel<MODE, 2, TT, 1, 4, TT == 1 ? 2 : 3, TT == 1 ? 4 : 2>};
         if (waves >= 1024 || kb < 4) return Form{64, 256, stream_kernel<MODE, 1, TT, 1, 4, TT == 1 ? 8 : 4, 2>};
         if (waves >= 512 || kb < 8) return Form{32, 256, stream_kernel<MODE, 1, TT, 2, 4, 4, 2>};
@@ -608,8 +661,18 @@ static Form stream_form(uint32_t out, uint32_t kb, uint64_t tiles) {
         return Form{16, 512, stream_kernel<MODE, 1, TT, 8, 8, 4, 2>};
     }
 }
+
+static hipError_t launch_form(Prof *p, hipStream_t s, const char *name, const Form &f, uint64_t tiles, q8::Args a) {
+    a.col_tiles = (a.out + f.cols - 1) / f.cols;
+    const uint64_t blocks = (tiles * a.col_tiles + q8::kXcds - 1) / q8::kXcds * q8::kXcds;
+    if (blocks > 0x7fffffffull) return hipErrorInvalidConfiguration;
+    return launch_kernel(p, name, f.kernel, dim3((uint32_t)blocks), dim3(f.threads), 0, s, a);
+}
+
+// scratch: F32 values for the two-launch SwiGLU of few positions
 template <int MODE>
-static hipError_t launch_q8(Prof *p, hipStream_t s, const char *name, q8::Args a) {
+static hipError_t launch_q8(Prof *p, hipStream_t s, const char *name, q8::Args a, float *scratch = nullptr,
+                            uint64_t scratch_len = 0) {
     using namespace q8;
     a.kb = (a.in + 127) / 128;
     const uint32_t experts = a.offsets ? a.experts : 1;
@@ -619,16 +682,27 @@ static hipError_t launch_q8(Prof *p, hipStream_t s, const char *name, q8::Args a
     };
     // DMA offsets are 32-bit
     const bool tiled = a.P > 32ull * experts && (uint64_t)a.xrows * a.in < 0xffffffffull;
-    const bool two = a.P > 8ull * experts;
-    const uint32_t bm = tiled ? (MODE == F32OUT ? 64 : 128) : two && !(experts == 1 && a.P <= 16) ? 32 : 16;
+    const bool two = a.P > 8ull * experts && !(experts == 1 && a.P <= 16);
+    const uint32_t bm = tiled ? (MODE == F32OUT ? 64 : 128) : two ? 32 : 16;
     const uint64_t tiles = max_tiles(bm);
-    const Form f = tiled      ? Form{MODE == SWIGLU ? 128u : 256u, 256, tile_kernel<MODE, MODE == F32OUT ? 4 : 8>}
-                   : bm == 32 ? stream_form<MODE, 2>(a.out, a.kb, tiles)
-                              : stream_form<MODE, 1>(a.out, a.kb, tiles);
-    a.col_tiles = (a.out + f.cols - 1) / f.cols;
-    const uint64_t blocks = (tiles * a.col_tiles + kXcds - 1) / kXcds * kXcds;
-    if (blocks > 0x7fffffffull) return hipErrorInvalidConfiguration;
-    return launch_kernel(p, name, f.kernel, dim3((uint32_t)blocks), dim3(f.threads), 0, s, a);
+    if constexpr (MODE == SWIGLU) {
+        // Blocks of 128 outputs (512 KiB of weights at 2048 columns) leave most
+        // of the CUs idle when there are few: then blocks of 16 to 64 outputs
+        // write F32 rows, and a second launch quantises them.
+        if (!tiled && tiles * ((a.out + 127) / 128) <= kSplitBlocks && (uint64_t)a.P * a.out <= scratch_len) {
+            Args b = a;
+            b.y = scratch;
+            const hipError_t e = launch_form(p, s, name, two ? stream_form<ACT, 2>(a.out, a.kb, tiles)
+                                                             : stream_form<ACT, 1>(a.out, a.kb, tiles), tiles, b);
+            if (e != hipSuccess) return e;
+            return launch_kernel(p, "quantize_q8", quantize_kernel, dim3(a.P), dim3(kThreads), 0, s, a,
+                                 (const float *)scratch);
+        }
+    }
+    const Form f = tiled ? Form{MODE == SWIGLU ? 128u : 256u, 256, tile_kernel<MODE, MODE == F32OUT ? 4 : 8>}
+                   : two ? stream_form<MODE, 2>(a.out, a.kb, tiles)
+                         : stream_form<MODE, 1>(a.out, a.kb, tiles);
+    return launch_form(p, s, name, f, tiles, a);
 }
 
 hipError_t launch_q8_rows(Prof *p, hipStream_t s, const char *name, const Q8Weight &w, const Q8Rows &x,
@@ -641,14 +715,15 @@ hipError_t launch_q8_rows(Prof *p, hipStream_t s, const char *name, const Q8Weig
 }
 
 hipError_t launch_q8_swiglu(Prof *p, hipStream_t s, const Q8Weight &gate, const Q8Weight &up, const Q8Rows &x,
-                            const uint32_t *offsets, const uint32_t *perm, uint32_t k, const Q8Rows &out) {
+                            const uint32_t *offsets, const uint32_t *perm, uint32_t k, const Q8Rows &out,
+                            float *scratch, uint64_t scratch_len) {
     q8::Args a{};
     a.w = gate.codes, a.ws = gate.scales, a.w2 = up.codes, a.ws2 = up.scales, a.stype = gate.stype;
     a.in = gate.in, a.out = gate.out, a.experts = gate.experts;
     a.x = x.codes, a.xs = x.scales, a.xrows = x.rows, a.P = out.rows;
     a.offsets = offsets, a.perm = perm, a.kdiv = k;
     a.codes = out.codes, a.scales = out.scales;
-    return launch_q8<q8::SWIGLU>(p, s, "expert_swiglu_q8", a);
+    return launch_q8<q8::SWIGLU>(p, s, "expert_swiglu_q8", a, scratch, scratch_len);
 }
 
 }  // namespace moehip

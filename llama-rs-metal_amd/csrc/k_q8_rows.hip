@@ -14,13 +14,6 @@ namespace moehip {
 // where that is written: it may be x or the residual itself).
 constexpr uint32_t kQ8NormThreads = 256, kQ8NormHold = 2;
 
-__device__ __forceinline__ uint32_t row16_max(uint32_t v) {
-    v = max(v, dpp_u<kDppQuad1>(v));
-    v = max(v, dpp_u<kDppQuad2>(v));
-    v = max(v, dpp_u<kDppHalfMirror>(v));
-    return max(v, dpp_u<kDppMirror>(v));
-}
-
 template <int T, bool VEC>
 __global__ __launch_bounds__(kQ8NormThreads) void norm_q8_kernel(const float *x, const float *resid, const void *w,
                                                                  float *sum, float *y, uint8_t *codes,

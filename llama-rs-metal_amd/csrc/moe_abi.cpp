@@ -81,7 +81,8 @@ moe_status moe_gpu_create(int device, moe_gpu **out) {
         hipEventCreateWithFlags(&g->ev_fork, hipEventDisableTiming) != hipSuccess ||
         hipEventCreateWithFlags(&g->ev_join, hipEventDisableTiming) != hipSuccess ||
         hipMalloc(reinterpret_cast<void **>(&g->arrive), 256) != hipSuccess ||
-        zero_new(g, g->arrive, 256) != hipSuccess) {
+        zero_new(g, g->arrive, 256) != hipSuccess ||
+        hipMalloc(reinterpret_cast<void **>(&g->q8_rows), kQ8RowsLen * 4) != hipSuccess) {
         if (g->arrive) (void)hipFree(g->arrive);
         delete g;
         return MOE_ERR_GPU;
@@ -106,6 +107,7 @@ void moe_gpu_destroy(moe_gpu *g) {
     }
     for (auto e : g->prof.pool) (void)hipEventDestroy(e);
     (void)hipFree(g->arrive);
+    (void)hipFree(g->q8_rows);
     (void)hipEventDestroy(g->ev_begin);
     (void)hipEventDestroy(g->ev_end);
     (void)hipEventDestroy(g->ev_fork);

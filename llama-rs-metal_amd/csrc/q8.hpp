@@ -25,6 +25,14 @@ __device__ __forceinline__ uint32_t bf16_bits(float x) {
     return abs_word(x) > 0x7f800000u ? (b >> 16) | 0x40u : (b + 0x7fffu + ((b >> 16) & 1u)) >> 16;
 }
 
+// The maximum over each aligned row of 16 lanes, all of which are active.
+__device__ __forceinline__ uint32_t row16_max(uint32_t v) {
+    v = max(v, dpp_u<kDppQuad1>(v));
+    v = max(v, dpp_u<kDppQuad2>(v));
+    v = max(v, dpp_u<kDppHalfMirror>(v));
+    return max(v, dpp_u<kDppMirror>(v));
+}
+
 // The stored scale of 128 values whose largest magnitude (abs_word) is `top`.
 // A group that holds an infinity or a NaN gets a scale of infinity or NaN, so
 // each of its values reads back as NaN (0 * inf, NaN * inf).
