@@ -23,6 +23,8 @@
 // holds token c and four rows 4q + i.  A wave owns 64 weight rows as four
 // row tiles whose rows interleave, so that a lane's results over its tiles are
 // neighbouring outputs of one token.
+#include <type_traits>
+
 #include "q8.hpp"
 
 namespace moehip {
@@ -33,9 +35,7 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 
-constexpr int kThreads = 256, kWaves = 4;
-constexpr int kWaveRows = 64;                     // weight rows per wave
-constexpr int kBlockRows = kWaveRows * kWaves;    // and per block
+constexpr int kThreads = 256;  // of the quantising launch
 
 enum { SWIGLU = 0, F32OUT = 1, BF16OUT = 2, ACT = 3 };  // ACT: SwiGLU as F32 rows
 
@@ -53,20 +53,20 @@ struct Args {
     uint32_t col_tiles;           // tiles along the outputs
 };
 
-// The work of this block: one of the M-tiles (runs of BM positions of a segment,
-// experts ascending) times one column tile.  Workgroup b runs on XCD b % 8; the
-// items are split into eight contiguous ranges, one per XCD, so the tiles that
-// share an expert's weights and a run's rows meet in one L2.  Every thread of the
-// block calls it; false (for all) where there is no item left.  Offsets past P
-// count as P and a segment that ends before it starts is empty.
+// The work of a block: items, each an M-tile (a run of at most BM positions of a
+// segment, experts ascending) times a column tile.  Workgroup b runs on XCD
+// b % 8; the items are split into eight contiguous ranges, one per XCD, so the
+// tiles that share an expert's weights and a run's rows meet in one L2; the
+// blocks of an XCD take its range's items in turn.  Every thread of the block
+// calls it; slots `from` and on of the block are written to out[0 .. n), at most
+// kMax; n is returned.  Offsets past P count as P and a segment that ends before
+// it starts is empty.
 struct Tile {
     uint32_t e, m0, end, ct;
 };
 constexpr uint32_t kXcds = 8;
-constexpr int kFind = 12;  // its words of LDS
 template <int BM, int NW>
-__device__ __forceinline__ bool find_tile(const Args &a, Tile &t, uint32_t *lds) {
-    static_assert(NW + 3 <= kFind, "LDS words");
+__device__ __forceinline__ uint32_t find_items(const Args &a, uint32_t from, uint32_t kMax, Tile *out, uint32_t *lds /* NW */) {
     const uint32_t tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     const uint32_t per = (a.experts + 64 * NW - 1) / (64 * NW), e0 = tid * per;
     auto seg = [&](uint32_t e, uint32_t &lo, uint32_t &n) {
@@ -99,31 +99,49 @@ __device__ __forceinline__ bool find_tile(const Args &a, Tile &t, uint32_t *lds)
         }
     }
     const uint64_t items = (uint64_t)total * a.col_tiles, range = (items + kXcds - 1) / kXcds;
-    const uint64_t item = blockIdx.x % kXcds * range + blockIdx.x / kXcds;
-    if (blockIdx.x / kXcds >= range || item >= items) return false;
-    const uint32_t tile = (uint32_t)(item / a.col_tiles);
-    t.ct = (uint32_t)(item - (uint64_t)tile * a.col_tiles);
+    const uint64_t lo_item = blockIdx.x % kXcds * range, hi_item = min(items, lo_item + range);
+    const uint32_t turn = gridDim.x / kXcds;
+    const uint64_t first = lo_item + blockIdx.x / kXcds + (uint64_t)from * turn;
+    if (first >= hi_item) return 0;
+    const uint32_t n = (uint32_t)min((uint64_t)kMax, (hi_item - first + turn - 1) / turn);
     if (!a.offsets) {
-        t.e = 0, t.m0 = tile * BM, t.end = min(a.P, t.m0 + BM);
-        return true;
-    }
-    if (tile >= before && tile < before + mine) {
-        for (uint32_t i = 0; i < per && e0 + i < a.experts; i++) {
-            uint32_t lo, n;
-            const uint32_t hi = seg(e0 + i, lo, n);
-            if (tile - before < n) {
-                lds[NW] = e0 + i;
-                lds[NW + 1] = lo + (tile - before) * BM;
-                lds[NW + 2] = hi;
-                break;
+        if (tid < n) {
+            const uint64_t item = first + (uint64_t)tid * turn;
+            const uint32_t tile = (uint32_t)(item / a.col_tiles), m0 = tile * BM;
+            out[tid] = Tile{0, m0, min(a.P, m0 + BM), (uint32_t)(item - (uint64_t)tile * a.col_tiles)};
+        }
+    } else {
+        for (uint32_t s = 0; s < n; s++) {
+            const uint64_t item = first + (uint64_t)s * turn;
+            const uint32_t tile = (uint32_t)(item / a.col_tiles);
+            if (tile < before || tile >= before + mine) continue;
+            uint32_t at = before;
+            for (uint32_t i = 0; i < per && e0 + i < a.experts; i++) {
+                uint32_t lo, k;
+                const uint32_t hi = seg(e0 + i, lo, k);
+                if (tile - at < k) {
+                    const uint32_t m0 = lo + (tile - at) * BM;
+                    out[s] = Tile{e0 + i, m0, min(hi, m0 + BM), (uint32_t)(item - (uint64_t)tile * a.col_tiles)};
+                    break;
+                }
+                at += k;
             }
-            before += n;
         }
     }
     __syncthreads();
-    t.e = __builtin_amdgcn_readfirstlane(lds[NW]);
-    t.m0 = __builtin_amdgcn_readfirstlane(lds[NW + 1]);
-    t.end = min(__builtin_amdgcn_readfirstlane(lds[NW + 2]), t.m0 + BM);
+    return n;
+}
+// The one item of a block in a grid with a block per item.
+constexpr int kFind = 12;  // its words of LDS
+template <int BM, int NW>
+__device__ __forceinline__ bool find_tile(const Args &a, Tile &t, uint32_t *lds) {
+    static_assert(NW + 4 <= kFind, "LDS words");
+    Tile *out = reinterpret_cast<Tile *>(lds + NW);
+    if (find_items<BM, NW>(a, 0, 1, out, lds) == 0) return false;
+    t.e = __builtin_amdgcn_readfirstlane(out->e);
+    t.m0 = __builtin_amdgcn_readfirstlane(out->m0);
+    t.end = __builtin_amdgcn_readfirstlane(out->end);
+    t.ct = __builtin_amdgcn_readfirstlane(out->ct);
     return true;
 }
 
@@ -172,53 +190,73 @@ __device__ __forceinline__ f32x4q block_dot(const Operand<true> &a, const Operan
 // The outputs of a wave's row tiles for NS token tiles of 16: acc[j][i] holds row
 // tile j, token tile i; the lane's rows are neighbours from `col` on; to[i] is
 // where the lane's token of tile i goes.
+typedef __bf16 bf16x2q __attribute__((ext_vector_type(2)));
+typedef float f32x2q __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {  // nearest even
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2q{a, b}, bf16x2q));
+}
 template <int MODE, int RT, int NS>
 __device__ __forceinline__ void store_rows(const Args &a, const f32x4q (&acc)[RT][NS], const uint32_t (&to)[NS],
                                            uint32_t col) {
-    // whole groups of four where every row starts aligned
-    const bool vec = a.out % 4 == 0 && (reinterpret_cast<uintptr_t>(a.y) & 15u) == 0;
+    // 16-byte stores of whole groups (4 F32, 8 bf16) where every row starts aligned
+    constexpr int G = MODE == BF16OUT && RT > 1 ? 8 : 4;
+    const bool vec = a.out % G == 0 && (reinterpret_cast<uintptr_t>(a.y) & 15u) == 0;
 #pragma unroll
     for (int i = 0; i < NS; i++) {
         if (to[i] == 0xffffffffu) continue;
         const uint64_t at = (uint64_t)to[i] * a.out + col;
+        if constexpr (MODE == F32OUT) {
+            float *y = static_cast<float *>(a.y) + at;
 #pragma unroll
-        for (int j = 0; j < RT; j++) {
-            const f32x4q v = acc[j][i];
-            const uint32_t cj = col + 4 * j;
-            if constexpr (MODE == F32OUT) {
-                float *y = static_cast<float *>(a.y) + at + 4 * j;
+            for (int j = 0; j < RT; j++) {
                 if (vec) {
-                    if (cj < a.out) *reinterpret_cast<f32x4q *>(y) = v;
+                    if (col + 4 * j < a.out) *reinterpret_cast<f32x4q *>(y + 4 * j) = acc[j][i];
                 } else {
 #pragma unroll
                     for (int r = 0; r < 4; r++)
-                        if (cj + r < a.out) y[r] = v[r];
+                        if (col + 4 * j + r < a.out) y[4 * j + r] = acc[j][i][r];
+                }
+            }
+        } else {
+            uint16_t *y = static_cast<uint16_t *>(a.y) + at;
+            uint32_t b[2 * RT];
+#pragma unroll
+            for (int j = 0; j < RT; j++) {
+                b[2 * j] = bf16_pair(acc[j][i][0], acc[j][i][1]);
+                b[2 * j + 1] = bf16_pair(acc[j][i][2], acc[j][i][3]);
+            }
+            if (vec) {
+                if constexpr (G == 8) {
+#pragma unroll
+                    for (int j = 0; j < RT; j += 2)
+                        if (col + 4 * j < a.out)
+                            *reinterpret_cast<u32x4q *>(y + 4 * j) = u32x4q{b[2 * j], b[2 * j + 1], b[2 * j + 2], b[2 * j + 3]};
+                } else {
+                    if (col < a.out) *reinterpret_cast<u32x2q *>(y) = u32x2q{b[0], b[1]};
                 }
             } else {
-                uint16_t *y = static_cast<uint16_t *>(a.y) + at + 4 * j;
-                uint32_t b[4];
 #pragma unroll
-                for (int r = 0; r < 4; r++) b[r] = bf16_bits(v[r]);
-                if (vec) {
-                    if (cj < a.out) *reinterpret_cast<u32x2q *>(y) = u32x2q{b[0] | b[1] << 16, b[2] | b[3] << 16};
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        if (cj + r < a.out) y[r] = (uint16_t)b[r];
-                }
+                for (int r = 0; r < 4 * RT; r++)
+                    if (col + r < a.out) y[r] = (uint16_t)(b[r / 2] >> (16 * (r % 2)));
             }
         }
     }
 }
 
-__device__ __forceinline__ float swiglu_of(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+// silu(g) * u; the exponential and the reciprocal are within 2^-22 of theirs,
+// far below the 2^-4 of the 8-bit codes this becomes
+__device__ __forceinline__ float swiglu_of(float g, float u) {
+    return g * __builtin_amdgcn_rcpf(1.0f + exp_fast(-g)) * u;
+}
 
 // SWIGLU: row tiles 0 .. RT/2 - 1 of acc are gate rows, the rest their up rows.
 // The waves of the block hold 128 output columns of its tokens: the largest
 // magnitude of each token goes through LDS (tops: [NW][BM]).
-template <int RT, int NS, int BM, int NW>
+// Token tile i is rows row0 + RS * i .. + 15 of the block's; `wv` the wave's place
+// among those that share tokens.
+template <int RT, int NS, int BM, int NW, int RS>
 __device__ __forceinline__ void store_swiglu(const Args &a, const f32x4q (&acc)[RT][NS], const uint32_t (&to)[NS],
-                                             uint32_t col, uint32_t ct, uint32_t wv, uint32_t *tops) {
+                                             uint32_t col, uint32_t ct, uint32_t wv, uint32_t row0, uint32_t *tops) {
     constexpr int V = 2 * RT;  // columns a lane holds
     const uint32_t lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4, ob = (a.out + 127) / 128;
     const bool cols_in = col < a.out;  // (out is a multiple of 16: all of the lane's columns or none)
@@ -233,12 +271,12 @@ __device__ __forceinline__ void store_swiglu(const Args &a, const f32x4q (&acc)[
             if (cols_in) top = max(top, abs_word(act[i][r]));
         }
         top = max_xor32_u(max_xor16_u(top));
-        if (q == 0) tops[wv * BM + 16 * i + c] = top;
+        if (q == 0) tops[wv * BM + row0 + RS * i + c] = top;
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < NS; i++) {
-        const uint32_t at = 16 * i + c;
+        const uint32_t at = row0 + RS * i + c;
         uint32_t top = tops[at];
 #pragma unroll
         for (int v = 1; v < NW; v++) top = max(top, tops[v * BM + at]);
@@ -266,7 +304,8 @@ __device__ __forceinline__ void store_swiglu(const Args &a, const f32x4q (&acc)[
 // kChunk blocks wait in LDS as F32, loaded before the codes so that their wait
 // leaves the codes in flight.
 constexpr uint32_t kChunk = 64;
-constexpr uint64_t kSplitBlocks = 512;
+constexpr uint64_t kCus = 256;
+constexpr uint64_t kSplitBlocks = 400;
 
 template <int MODE, int RT, int TT, int KS, int NW>
 struct StreamLds {
@@ -302,7 +341,7 @@ __global__ __launch_bounds__(64 * NW, WPS) void stream_kernel(Args a) {
 #pragma unroll
     for (int j = 0; j < RT; j++) {
         const uint32_t r = kGated ? n0 + c : n0 + 4 * RT * (c >> 2) + 4 * j + (c & 3);
-        woff[j] = (min(r, a.out - 1) - nb) * a.in + 16 * q;
+        woff[j] = (min(r, a.out - 1) - nb) * a.in;
     }
     // positions past the tile's end read its first row; outputs go to to[]
     auto source = [&](uint32_t p) -> uint32_t {
@@ -321,7 +360,7 @@ __global__ __launch_bounds__(64 * NW, WPS) void stream_kernel(Args a) {
             to[i] = live && pair / a.kdiv < a.xrows ? p : 0xffffffffu;
         else
             to[i] = live && pair < a.P ? pair : 0xffffffffu;
-        xrow[i] = a.x + (uint64_t)source(p) * a.in + 16 * q;
+        xrow[i] = a.x + (uint64_t)source(p) * a.in;
     }
     const uint64_t swrow = ((uint64_t)t.e * ob + min(n0 / 128, ob - 1)) * nk;
     f32x4q acc[RT][TT] = {};
@@ -339,17 +378,17 @@ __global__ __launch_bounds__(64 * NW, WPS) void stream_kernel(Args a) {
         Codes w[D][RT], x[D][TT];
         auto load = [&](int d, uint32_t kb) {  // blocks past the chunk's end: its last again, with a scale of zero
             const uint32_t k = k0 + min(kb, kn - 1), k128 = k * 128;
-            const bool last = tail && k + 1 == nk;
+            const bool last = tail && k + 1 == nk;  // chunks past `in` read the block's first
             const uint32_t lo = last && 16 * q >= tail ? 0 : 16 * q, hi = last && 16 * q + 64 >= tail ? 0 : 16 * q + 64;
 #pragma unroll
             for (int j = 0; j < RT; j++) {
                 const __amdgpu_buffer_rsrc_t r = kGated && j == 1 ? rw2 : rw;
-                w[d][j].lo = __builtin_bit_cast(u32x4q, __builtin_amdgcn_raw_buffer_load_b128(r, woff[j], k128, 0));
-                w[d][j].hi = __builtin_bit_cast(u32x4q, __builtin_amdgcn_raw_buffer_load_b128(r, woff[j] + 64, k128, 0));
+                w[d][j].lo = __builtin_bit_cast(u32x4q, __builtin_amdgcn_raw_buffer_load_b128(r, woff[j] + lo, k128, 0));
+                w[d][j].hi = __builtin_bit_cast(u32x4q, __builtin_amdgcn_raw_buffer_load_b128(r, woff[j] + hi, k128, 0));
             }
 #pragma unroll
             for (int i = 0; i < TT; i++) {
-                const uint8_t *row = xrow[i] - 16 * q + k128;
+                const uint8_t *row = xrow[i] + k128;
                 x[d][i].lo = *reinterpret_cast<const u32x4q *>(row + lo);
                 x[d][i].hi = *reinterpret_cast<const u32x4q *>(row + hi);
             }
@@ -413,7 +452,7 @@ __global__ __launch_bounds__(64 * NW, WPS) void stream_kernel(Args a) {
                     acc[j][i] += *reinterpret_cast<const f32x4q *>(lds.red[rg * (KS - 1) + v] + ((j * TT + i) * 64 + lane) * 4);
     }
     if constexpr (MODE == SWIGLU)
-        store_swiglu<RT, TT, BM, NW>(a, acc, to, n0 + 4 * q, t.ct, wv, lds.tops);
+        store_swiglu<RT, TT, BM, NW, 16>(a, acc, to, n0 + 4 * q, t.ct, wv, 0, lds.tops);
     else if constexpr (MODE == ACT) {
         if (n0 + 4 * q >= a.out) return;  // (out is a multiple of 16)
 #pragma unroll
@@ -428,174 +467,242 @@ __global__ __launch_bounds__(64 * NW, WPS) void stream_kernel(Args a) {
         store_rows<MODE, RT, TT>(a, acc, to, n0 + 4 * RT * q);
 }
 
-// The same product for many rows per expert: a block of 128 (64 for F32 outputs)
-// tokens.  The token rows of a block of 128 columns reach LDS by buffer DMA
-// (eight rows of 128 bytes an instruction, 16-byte chunks XOR-swizzled by half
-// the row number so that 16 rows' equal chunks lie in distinct banks), double
-// buffered, one barrier a step; the weights go from memory straight to the
-// waves' registers, one step ahead (no two waves share a weight row).  The
-// rows' and weights' scales of 16 steps wait in LDS as F32.
+// The same product for many rows per expert: items of 128 tokens and 256 weight
+// rows (SWIGLU: 128 gate rows and their up rows) for blocks of eight waves, one
+// a CU, that take one item after another.  A step is a block of 128 columns: its
+// token and weight rows reach LDS by buffer DMA (eight rows of 128 bytes an
+// instruction, so that neighbouring lanes read neighbouring bytes: loads in
+// the matrix cores' own layout, 16 rows an instruction, took four times as long),
+// two steps ahead and across the items' borders; 16-byte chunks are XOR-swizzled
+// by half the row number, so that 16 rows' equal chunks lie in distinct banks.
+// The waves form 4 x 2: 64 weight rows times 64 tokens (every other tile of 16)
+// each, so that LDS is read 2 x 64 rows of 128 bytes for 16 matrix instructions.  One barrier a step.
+// The rows an item reads and writes are looked up once for kSlots items.
 typedef __attribute__((address_space(3))) void *lds_ptr;
-constexpr int kGroup = 16;  // steps whose scales are in LDS together
+constexpr int kGroup = 8, kStages = 3, kTileWaves = 8, kTileRows = 128, kTileCols = 256, kSlots = 8;
 
-template <int BM>
 struct TileLds {
-    uint8_t x[2][BM * 128];
-    float sx[2][kGroup][BM];
-    float sw[2][2][kGroup];
-    uint32_t tops[kWaves * BM];
-    uint32_t find[kFind];
+    uint8_t x[kStages][kTileRows * 128];
+    uint8_t w[kStages][kTileCols * 128];
+    uint16_t sx[3][kGroup][kTileRows];  // scales of kGroup steps: the current ones, the next, and those being stored
+    float sw[3][2][kGroup];
+    uint32_t tops[4 * kTileRows];
+    uint32_t map[kSlots][kTileRows];  // SWIGLU: input row of each position; else its output row; 0xffffffff: none
+    Tile slot[kSlots];
+    uint32_t scan[kTileWaves];
 };
 
-template <int MODE, int TT, int NS>
-__device__ __forceinline__ void tile_body(const Args &a, const Tile &t, TileLds<16 * TT> &lds) {
+template <int MODE>
+__global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
     constexpr bool kF16 = MODE == F32OUT;
-    constexpr int BM = 16 * TT, ND = NS / 2;  // ND: DMA instructions a wave issues per step
-    static_assert(NS % 2 == 0, "32 rows a round of DMA");
+    constexpr int NX = 2, NW = 4;     // DMA instructions of a wave and step: token rows, weight rows
+    constexpr int kLoads = NX + NW;
+    __shared__ __attribute__((aligned(16))) TileLds lds;
     const uint32_t tid = threadIdx.x, lane = tid & 63, c = lane & 15, q = lane >> 4;
-    const uint32_t wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t n0 = MODE == SWIGLU ? t.ct * (kBlockRows / 2) + wv * 32 : t.ct * kBlockRows + wv * kWaveRows;
-    const uint32_t nb = min(n0, a.out - 1);
-    const uint32_t nk = a.kb, tail = a.in % 128;
-    // weights: one resource per matrix from row nb on, a lane's four rows as offsets
-    const uint64_t wbase = ((uint64_t)t.e * a.out + nb) * a.in;
-    const uint32_t wbytes = (uint32_t)min((uint64_t)(a.out - nb) * a.in, (uint64_t)0xffffffffu);
-    const __amdgpu_buffer_rsrc_t rw = buffer_rsrc(a.w + wbase, wbytes);
-    const __amdgpu_buffer_rsrc_t rw2 = MODE == SWIGLU ? buffer_rsrc(a.w2 + wbase, wbytes) : rw;
-    uint32_t woff[4];
+    const uint32_t wv = __builtin_amdgcn_readfirstlane(tid >> 6), wg = wv >> 1, tg = wv & 1;
+    const uint32_t nk = a.kb, tail = a.in % 128, ob = (a.out + 127) / 128;
+    const __amdgpu_buffer_rsrc_t rx = buffer_rsrc(a.x, (uint32_t)((uint64_t)a.xrows * a.in));
+    const uint32_t wbytes = (uint32_t)((uint64_t)a.out * a.in);
+    // DMA: instruction i of wave wv fills LDS rows 8 (8 i + wv) .. + 7; lane l
+    // writes chunk l % 8 of row l / 8.  LDS row 64 g + 16 j + c holds the row that is
+    // row c of row tile j of the waves of group g: four row tiles interleave, so that a
+    // lane's results are neighbouring outputs (SWIGLU: tiles 0, 1 gate, 2, 3 up).
+    const uint32_t drow = 8 * wv + lane / 8;  // + 64 i
+    const uint32_t dchunk = ((lane % 8) ^ ((drow >> 1) & 7)) * 16;
+    const uint32_t dc = drow % 16, dj = drow / 16 % 4;
+    const uint32_t dlocal = MODE == SWIGLU ? 8 * (dc >> 2) + 4 * (dj & 1) + (dc & 3) : 16 * (dc >> 2) + 4 * dj + (dc & 3);
+    // the item whose steps are being loaded
+    __amdgpu_buffer_rsrc_t rw = rx;
+    uint32_t xoff[NX] = {}, woff[NW] = {};
+    auto aim = [&](uint32_t s) {
+        const Tile t = lds.slot[s];
+        const uint32_t e = __builtin_amdgcn_readfirstlane(t.e);
+        const uint8_t *w = MODE == SWIGLU && wv >= 4 ? a.w2 : a.w;  // (SWIGLU: the wave's rows are all of one matrix)
+        rw = buffer_rsrc(w + (uint64_t)e * a.out * a.in, wbytes);
+        // rows past `out` repeat the last and are not stored
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const uint32_t r = MODE == SWIGLU ? n0 + 8 * (c >> 2) + 4 * (j & 1) + (c & 3) : n0 + 16 * (c >> 2) + 4 * j + (c & 3);
-        woff[j] = (min(r, a.out - 1) - nb) * a.in + 16 * q;
-    }
-    // the source row of position p (any valid row past the tile's end) and where its outputs go
-    auto source = [&](uint32_t p) -> uint32_t {
-        const uint32_t pp = p < t.end ? p : t.m0;
-        if (MODE != SWIGLU) return pp;
-        return min((a.perm ? a.perm[pp] : pp) / a.kdiv, a.xrows - 1);
+        for (int i = 0; i < NW; i++)
+            woff[i] = min((MODE == SWIGLU ? t.ct * 128 + 32 * i : t.ct * 256 + 64 * i) + dlocal, a.out - 1) * a.in + dchunk;
+        // positions past the item's end, and those that name no row, read some row
+#pragma unroll
+        for (int i = 0; i < NX; i++) {
+            const uint32_t r = drow + 64 * i, p = t.m0 + r;
+            const uint32_t src = MODE == SWIGLU ? min(lds.map[s][r], a.xrows - 1) : p < t.end ? p : t.m0;
+            xoff[i] = src * a.in + dchunk;
+        }
     };
-    uint32_t to[NS];
+    // columns past `in` in the last step: a chunk is replaced by its row's first of
+    // the block, and the weights' codes are zeroed when they are used
+    const uint32_t back = tail && dchunk >= tail ? dchunk : 0;
+    auto load = [&](uint32_t stage, uint32_t kb) {
+        const uint32_t b = kb + 1 == nk ? back : 0;
 #pragma unroll
-    for (int i = 0; i < NS; i++) {
-        const uint32_t p = t.m0 + 16 * i + c;
-        const bool live = p < t.end;
-        const uint32_t pair = a.perm ? a.perm[live ? p : t.m0] : p;
-        if (MODE == SWIGLU)
-            to[i] = live && pair / a.kdiv < a.xrows ? p : 0xffffffffu;
-        else
-            to[i] = live && pair < a.P ? pair : 0xffffffffu;
-    }
-    const __amdgpu_buffer_rsrc_t rx = buffer_rsrc(a.x, (uint32_t)min((uint64_t)a.xrows * a.in, (uint64_t)0xffffffffu));
-    uint32_t xoff[ND], xlast[ND];  // of a step's 16 bytes, and of the last step's (past `in`: the block's first)
+        for (int i = 0; i < NX; i++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lds_ptr)(lds.x[stage] + (64 * i + 8 * wv) * 128), 16,
+                                                     xoff[i] - b, kb * 128, 0, 0);
 #pragma unroll
-    for (int i = 0; i < ND; i++) {
-        const uint32_t r = 8 * (kWaves * i + wv) + lane / 8, chunk = (lane % 8) ^ ((r >> 1) & 7);
-        const uint32_t base = source(t.m0 + r) * a.in;
-        xoff[i] = base + 16 * chunk;
-        xlast[i] = tail && 16 * chunk >= tail ? base : xoff[i];
-    }
-    // the thread's share of the rows' scales of 16 steps: one row, kSr neighbouring steps
-    constexpr int kSr = BM * kGroup / kThreads;
+        for (int i = 0; i < NW; i++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_ptr)(lds.w[stage] + (64 * i + 8 * wv) * 128), 16, woff[i] - b,
+                                                     kb * 128, 0, 0);
+    };
+    // the thread's share of the scales of kGroup steps: kSr neighbouring steps of one row
+    constexpr int kSr = kTileRows * kGroup / (64 * kTileWaves);
     const uint32_t srow = tid / (kGroup / kSr), sk = tid % (kGroup / kSr) * kSr;
-    const uint16_t *sxp = a.xs + (uint64_t)source(t.m0 + srow) * nk;
-    const uint32_t ob = (a.out + 127) / 128;
     const bool has_sw = tid < 2 * kGroup;
-    const uint32_t swb = MODE == SWIGLU ? t.ct : min(2 * t.ct + tid / kGroup, ob - 1);
-    const void *swp = MODE == SWIGLU && tid >= kGroup ? a.ws2 : a.ws;
-    const uint64_t swrow = ((uint64_t)t.e * ob + swb) * nk;
     uint16_t sr[kSr];
     float swr = 0.f;
-    auto load_scales = [&](uint32_t k0) {
+    auto load_scales = [&](uint32_t s, uint32_t k0) {
+        const Tile t = lds.slot[s];
+        const uint32_t p = t.m0 + srow;
+        const uint32_t src = MODE == SWIGLU ? min(lds.map[s][srow], a.xrows - 1) : p < t.end ? p : t.m0;
 #pragma unroll
-        for (int i = 0; i < kSr; i++) sr[i] = sxp[min(k0 + sk + i, nk - 1)];
-        if (has_sw) swr = scale_at(swp, a.stype, swrow + min(k0 + tid % kGroup, nk - 1));
+        for (int i = 0; i < kSr; i++) sr[i] = a.xs[(uint64_t)src * nk + min(k0 + sk + i, nk - 1)];
+        const uint32_t b = MODE == SWIGLU ? t.ct : min(2 * t.ct + tid / kGroup, ob - 1);
+        const void *from = MODE == SWIGLU && tid >= kGroup ? a.ws2 : a.ws;
+        if (has_sw) swr = scale_at(from, a.stype, ((uint64_t)t.e * ob + b) * nk + min(k0 + tid % kGroup, nk - 1));
     };
     auto keep_scales = [&](uint32_t buf) {
 #pragma unroll
-        for (int i = 0; i < kSr; i++) lds.sx[buf][sk + i][srow] = bf16_to_f32(sr[i]);
+        for (int i = 0; i < kSr; i++) lds.sx[buf][sk + i][srow] = sr[i];
         if (has_sw) lds.sw[buf][tid / kGroup][tid % kGroup] = swr;
     };
-    auto dma = [&](uint32_t buf, uint32_t kb) {
-#pragma unroll
-        for (int i = 0; i < ND; i++)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lds_ptr)(lds.x[buf] + 8 * (kWaves * i + wv) * 128), 16,
-                                                     kb + 1 == nk ? xlast[i] : xoff[i], kb * 128, 0, 0);
+    // a lane's chunks of its row in tile 0 of a wave's rows
+    const uint32_t lo = c * 128 + ((q ^ (c >> 1)) << 4), hi = c * 128 + (((q + 4) ^ (c >> 1)) << 4);
+    const uint8_t *const xbase = lds.x[0] + 16 * tg * 128, *const wbase = lds.w[0] + 64 * wg * 128;
+    auto codes = [&](const uint8_t *rows) {
+        return Codes{*reinterpret_cast<const u32x4q *>(rows + lo), *reinterpret_cast<const u32x4q *>(rows + hi)};
     };
-    auto load_w = [&](Codes (&w)[4], uint32_t kb) {
+    // a step over the wave's first NS token tiles (tile i: rows 32 i + 16 tg on)
+    auto compute = [&](auto &acc, uint32_t stage, uint32_t kb, uint32_t grp) {
+        constexpr int NS = sizeof(acc[0]) / sizeof(acc[0][0]);
+        const uint8_t *xr = xbase + stage * (kTileRows * 128), *wr = wbase + stage * (kTileCols * 128);
+        const float sw = lds.sw[grp][MODE == SWIGLU ? 0 : wg >> 1][kb % kGroup];
+        const float sw2 = MODE == SWIGLU ? lds.sw[grp][1][kb % kGroup] : sw;
+        const uint16_t *sx = lds.sx[grp][kb % kGroup] + 16 * tg + c;
+        Codes wc[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const __amdgpu_buffer_rsrc_t r = MODE == SWIGLU && j >= 2 ? rw2 : rw;
-            w[j].lo = __builtin_bit_cast(u32x4q, __builtin_amdgcn_raw_buffer_load_b128(r, woff[j], kb * 128, 0));
-            w[j].hi = __builtin_bit_cast(u32x4q, __builtin_amdgcn_raw_buffer_load_b128(r, woff[j] + 64, kb * 128, 0));
-        }
-    };
-    f32x4q acc[4][NS] = {};
-    Codes w[4], wn[4];
-    load_scales(0);
-    dma(0, 0);
-    load_w(w, 0);
-    for (uint32_t kb = 0; kb < nk; kb++) {
-        const uint32_t buf = kb & 1, grp = kb / kGroup & 1;
-        if (kb % kGroup == 0) keep_scales(grp);
-        __builtin_amdgcn_s_waitcnt(0);  // this step's DMA, codes and scales are here
-        __syncthreads();                // everyone's; and everyone is done with the other buffers
-        if (kb + 1 < nk) {
-            if ((kb + 1) % kGroup == 0) load_scales(kb + 1);
-            dma(buf ^ 1, kb + 1);
-            load_w(wn, kb + 1);
-        }
+        for (int j = 0; j < 4; j++) wc[j] = codes(wr + j * 2048);
         if (tail && kb + 1 == nk) {
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                if (16 * q >= tail) w[j].lo = u32x4q{0, 0, 0, 0};
-                if (16 * q + 64 >= tail) w[j].hi = u32x4q{0, 0, 0, 0};
+                if (16 * q >= tail) wc[j].lo = u32x4q{0, 0, 0, 0};
+                if (16 * q + 64 >= tail) wc[j].hi = u32x4q{0, 0, 0, 0};
             }
         }
-        const Operand<kF16> wo[4] = {Operand<kF16>(w[0]), Operand<kF16>(w[1]), Operand<kF16>(w[2]), Operand<kF16>(w[3])};
-        const uint32_t wsel = MODE == SWIGLU ? 0 : wv >> 1;
-        const float sw = lds.sw[grp][wsel][kb % kGroup];
-        const float sw2 = MODE == SWIGLU ? lds.sw[grp][1][kb % kGroup] : sw;
+        const Operand<kF16> wo[4] = {Operand<kF16>(wc[0]), Operand<kF16>(wc[1]), Operand<kF16>(wc[2]), Operand<kF16>(wc[3])};
+        // A block's sums join their running sums kLag products later, and a
+        // token tile is read one tile ahead, in this order: the matrix cores
+        // then wait for neither.
+        constexpr int kLag = 3;
+        Codes xc[NS];
+        float s1[NS], s2[NS];
+        f32x4q d[4 * NS];
+        xc[0] = codes(xr);
+        s1[0] = bf16_to_f32(sx[0]);
 #pragma unroll
-        for (int i = 0; i < NS; i++) {
-            const uint32_t r = 16 * i + c, sz = (r >> 1) & 7;
-            Codes xc;
-            xc.lo = *reinterpret_cast<const u32x4q *>(&lds.x[buf][r * 128 + ((q ^ sz) << 4)]);
-            xc.hi = *reinterpret_cast<const u32x4q *>(&lds.x[buf][r * 128 + (((q + 4) ^ sz) << 4)]);
-            const float sx = lds.sx[grp][kb % kGroup][r];
-            const Operand<kF16> xo(xc);
-            const float s1 = sx * sw, s2 = MODE == SWIGLU ? sx * sw2 : s1;
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const f32x4q d = block_dot(wo[j], xo);
-                const float s = j >= 2 ? s2 : s1;
-#pragma unroll
-                for (int e = 0; e < 4; e++) acc[j][i][e] = fmaf(d[e], s, acc[j][i][e]);
+        for (int n = 0; n < 4 * NS + kLag; n++) {
+            const int i = n / 4, j = n % 4;
+            if (n < 4 * NS) {
+                if (j == 0) {
+                    if (i + 1 < NS) {
+                        xc[i + 1] = codes(xr + (i + 1) * 4096);
+                        s1[i + 1] = bf16_to_f32(sx[32 * (i + 1)]);
+                    }
+                    s2[i] = MODE == SWIGLU ? s1[i] * sw2 : 0.f;
+                    s1[i] *= sw;
+                }
+                d[n] = block_dot(wo[j], Operand<kF16>(xc[i]));
             }
-        }
+            if (n >= kLag) {
+                const int m = n - kLag;
+                const float s = MODE == SWIGLU && m % 4 >= 2 ? s2[m / 4] : s1[m / 4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) w[j] = wn[j];
-    }
-    if constexpr (MODE == SWIGLU)
-        store_swiglu<4, NS, BM, kWaves>(a, acc, to, n0 + 8 * q, t.ct, wv, lds.tops);
-    else
-        store_rows<MODE, 4, NS>(a, acc, to, n0 + 16 * q);
-}
-
-template <int MODE, int TT>
-__global__ __launch_bounds__(kThreads, 2) void tile_kernel(Args a) {
-    __shared__ __attribute__((aligned(16))) TileLds<16 * TT> lds;
-    Tile t;
-    if (!find_tile<16 * TT, kWaves>(a, t, lds.find)) return;
-    // token tiles in use, in steps of a quarter (32 rows of 128)
-    const uint32_t live = t.end - t.m0;
-    if constexpr (TT == 8) {
-        if (live > 96) tile_body<MODE, TT, 8>(a, t, lds);
-        else if (live > 64) tile_body<MODE, TT, 6>(a, t, lds);
-        else if (live > 32) tile_body<MODE, TT, 4>(a, t, lds);
-        else tile_body<MODE, TT, 2>(a, t, lds);
-    } else {
-        if (live > 32) tile_body<MODE, TT, 4>(a, t, lds);
-        else tile_body<MODE, TT, 2>(a, t, lds);
+                for (int e = 0; e < 4; e++) acc[m % 4][m / 4][e] = fmaf(d[m][e], s, acc[m % 4][m / 4][e]);
+            }
+            if constexpr (!kF16) __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    for (uint32_t from = 0;; from += kSlots) {
+        const uint32_t slots = find_items<kTileRows, kTileWaves>(a, from, kSlots, lds.slot, lds.scan);
+        if (slots == 0) return;
+        for (uint32_t i = tid; i < slots * kTileRows; i += 64 * kTileWaves) {
+            const Tile t = lds.slot[i / kTileRows];
+            const uint32_t p = t.m0 + i % kTileRows;
+            uint32_t to = 0xffffffffu;
+            if (p < t.end) {
+                to = a.perm ? a.perm[p] : p;
+                if constexpr (MODE == SWIGLU) to /= a.kdiv;
+                if (to >= (MODE == SWIGLU ? a.xrows : a.P)) to = 0xffffffffu;
+            }
+            lds.map[i / kTileRows][i % kTileRows] = to;
+        }
+        __syncthreads();
+        // the step that is loaded next: slot ps (past the last: the last again,
+        // unused), block pk; the stage it goes to; its scales' buffer
+        uint32_t ps = 0, pk = 0, pstage = 0, pgrp = 2, grp = 2, stage = 0;
+        bool pending = false;
+        auto ahead = [&] {
+            if (pk == 0) aim(min(ps, slots - 1));
+            if (pk % kGroup == 0) {  // (before the step's own loads, whose wait then covers them)
+                load_scales(min(ps, slots - 1), pk);
+                pending = true;
+                pgrp = pgrp == 2 ? 0 : pgrp + 1;
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            load(pstage, pk);
+            pstage = pstage == kStages - 1 ? 0 : pstage + 1;
+            if (++pk == nk) pk = 0, ps++;
+        };
+        auto store_scales = [&] {
+            if (pending) keep_scales(pgrp);
+            pending = false;
+        };
+        ahead();
+        store_scales();
+        ahead();
+        // slot s over the first NS token tiles of each wave
+        auto item = [&](auto tiles, uint32_t s) {
+            constexpr int NS = decltype(tiles)::value;
+            f32x4q acc[4][NS] = {};
+            for (uint32_t kb = 0; kb < nk; kb++) {
+                if (kb % kGroup == 0) grp = grp == 2 ? 0 : grp + 1;
+                // a step begins when its rows are in LDS: all but the loads of the step
+                // after it have landed (gfx9 encoding: vmcnt, then lgkmcnt 0 for the
+                // scales), everyone's, and nobody reads the buffer that is filled next
+                __builtin_amdgcn_sched_barrier(0);
+                __builtin_amdgcn_s_waitcnt(kLoads | (7 << 4) | (15 << 8));
+                store_scales();
+                __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4) | (0 << 8));
+                __builtin_amdgcn_s_barrier();
+                __builtin_amdgcn_sched_barrier(0);
+                ahead();
+                compute(acc, stage, kb, grp);
+                stage = stage == kStages - 1 ? 0 : stage + 1;
+            }
+            const Tile t = lds.slot[s];
+            const uint32_t ct = __builtin_amdgcn_readfirstlane(t.ct);
+            uint32_t to[NS];
+#pragma unroll
+            for (int i = 0; i < NS; i++) {
+                const uint32_t r = 32 * i + 16 * tg + c, m = lds.map[s][r];
+                to[i] = MODE == SWIGLU && m != 0xffffffffu ? t.m0 + r : m;
+            }
+            if constexpr (MODE == SWIGLU)
+                store_swiglu<4, NS, kTileRows, 4, 32>(a, acc, to, ct * 128 + wg * 32 + 8 * q, ct, wg, 16 * tg, lds.tops);
+            else
+                store_rows<MODE, 4, NS>(a, acc, to, ct * 256 + wg * 64 + 16 * q);
+        };
+        for (uint32_t s = 0; s < slots; s++) {
+            // (every wave takes the same way: the barriers are inside)
+            const uint32_t live = __builtin_amdgcn_readfirstlane(lds.slot[s].end - lds.slot[s].m0);
+            if (live > 96) item(std::integral_constant<int, 4>{}, s);
+            else if (live > 64) item(std::integral_constant<int, 3>{}, s);
+            else if (live > 32) item(std::integral_constant<int, 2>{}, s);
+            else item(std::integral_constant<int, 1>{}, s);
+        }
+        if (slots < kSlots) return;
+        __builtin_amdgcn_s_waitcnt(0);  // the loads past the last item have landed
+        __syncthreads();
     }
 }
 
@@ -662,9 +769,11 @@ static Form stream_form(uint32_t out, uint32_t kb, uint64_t tiles) {
     }
 }
 
-static hipError_t launch_form(Prof *p, hipStream_t s, const char *name, const Form &f, uint64_t tiles, q8::Args a) {
+static hipError_t launch_form(Prof *p, hipStream_t s, const char *name, const Form &f, uint64_t tiles, q8::Args a,
+                              uint64_t most_blocks = 0x7fffffff) {
     a.col_tiles = (a.out + f.cols - 1) / f.cols;
-    const uint64_t blocks = (tiles * a.col_tiles + q8::kXcds - 1) / q8::kXcds * q8::kXcds;
+    uint64_t blocks = (tiles * a.col_tiles + q8::kXcds - 1) / q8::kXcds * q8::kXcds;
+    if (blocks > most_blocks && most_blocks == q8::kCus) blocks = most_blocks;
     if (blocks > 0x7fffffffull) return hipErrorInvalidConfiguration;
     return launch_kernel(p, name, f.kernel, dim3((uint32_t)blocks), dim3(f.threads), 0, s, a);
 }
@@ -681,9 +790,9 @@ static hipError_t launch_q8(Prof *p, hipStream_t s, const char *name, q8::Args a
         return a.P / bm + (a.offsets ? (uint64_t)(experts < a.P ? experts : a.P) : (uint64_t)(a.P % bm != 0));
     };
     // DMA offsets are 32-bit
-    const bool tiled = a.P > 32ull * experts && (uint64_t)a.xrows * a.in < 0xffffffffull;
-    const bool two = a.P > 8ull * experts && !(experts == 1 && a.P <= 16);
-    const uint32_t bm = tiled ? (MODE == F32OUT ? 64 : 128) : two ? 32 : 16;
+    const bool tiled = a.P >= (a.offsets ? 8ull : 33ull) * experts && (uint64_t)a.xrows * a.in < 0xffffffffull && (uint64_t)a.out * a.in < 0xffffffffull;
+    const bool two = !a.offsets && a.P > 16;
+    const uint32_t bm = tiled ? 128 : two ? 32 : 16;
     const uint64_t tiles = max_tiles(bm);
     if constexpr (MODE == SWIGLU) {
         // Blocks of 128 outputs (512 KiB of weights at 2048 columns) leave most
@@ -699,10 +808,10 @@ static hipError_t launch_q8(Prof *p, hipStream_t s, const char *name, q8::Args a
                                  (const float *)scratch);
         }
     }
-    const Form f = tiled ? Form{MODE == SWIGLU ? 128u : 256u, 256, tile_kernel<MODE, MODE == F32OUT ? 4 : 8>}
+    const Form f = tiled ? Form{MODE == SWIGLU ? 128u : 256u, 512, tile_kernel<MODE>}
                    : two ? stream_form<MODE, 2>(a.out, a.kb, tiles)
                          : stream_form<MODE, 1>(a.out, a.kb, tiles);
-    return launch_form(p, s, name, f, tiles, a);
+    return launch_form(p, s, name, f, tiles, a, tiled ? kCus : 0x7fffffff);
 }
 
 hipError_t launch_q8_rows(Prof *p, hipStream_t s, const char *name, const Q8Weight &w, const Q8Rows &x,
