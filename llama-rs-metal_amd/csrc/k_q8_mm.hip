@@ -534,16 +534,15 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
     // columns past `in` in the last step: a chunk is replaced by its row's first of
     // the block, and the weights' codes are zeroed when they are used
     const uint32_t back = tail && dchunk >= tail ? dchunk : 0;
-    auto load = [&](uint32_t stage, uint32_t kb) {
+    // one of the kLoads instructions of block kb into `stage`
+    auto load = [&](int i, uint32_t stage, uint32_t kb) {
         const uint32_t b = kb + 1 == nk ? back : 0;
-#pragma unroll
-        for (int i = 0; i < NX; i++)
+        if (i < NX)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lds_ptr)(lds.x[stage] + (64 * i + 8 * wv) * 128), 16,
-                                                     xoff[i] - b, kb * 128, 0, 0);
-#pragma unroll
-        for (int i = 0; i < NW; i++)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_ptr)(lds.w[stage] + (64 * i + 8 * wv) * 128), 16, woff[i] - b,
-                                                     kb * 128, 0, 0);
+                                                     xoff[i < NX ? i : 0] - b, kb * 128, 0, 0);
+        else
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_ptr)(lds.w[stage] + (64 * (i - NX) + 8 * wv) * 128), 16,
+                                                     woff[i < NX ? 0 : i - NX] - b, kb * 128, 0, 0);
     };
     // the thread's share of the scales of kGroup steps: kSr neighbouring steps of one row
     constexpr int kSr = kTileRows * kGroup / (64 * kTileWaves);
@@ -572,8 +571,10 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
     auto codes = [&](const uint8_t *rows) {
         return Codes{*reinterpret_cast<const u32x4q *>(rows + lo), *reinterpret_cast<const u32x4q *>(rows + hi)};
     };
-    // a step over the wave's first NS token tiles (tile i: rows 32 i + 16 tg on)
-    auto compute = [&](auto &acc, uint32_t stage, uint32_t kb, uint32_t grp) {
+    // a step over the wave's first NS token tiles (tile i: rows 32 i + 16 tg on);
+    // the DMA of block lkb into lstage is issued between the products (in one
+    // go it held the waves up until the memory pipe had taken all of it)
+    auto compute = [&](auto &acc, uint32_t stage, uint32_t kb, uint32_t grp, uint32_t lstage, uint32_t lkb) {
         constexpr int NS = sizeof(acc[0]) / sizeof(acc[0][0]);
         const uint8_t *xr = xbase + stage * (kTileRows * 128), *wr = wbase + stage * (kTileCols * 128);
         const float sw = lds.sw[grp][MODE == SWIGLU ? 0 : wg >> 1][kb % kGroup];
@@ -612,6 +613,8 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
                     s1[i] *= sw;
                 }
                 d[n] = block_dot(wo[j], Operand<kF16>(xc[i]));
+#pragma unroll
+                for (int l = n * kLoads / (4 * NS); l < (n + 1) * kLoads / (4 * NS); l++) load(l, lstage, lkb);
             }
             if (n >= kLag) {
                 const int m = n - kLag;
@@ -641,17 +644,26 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
         // unused), block pk; the stage it goes to; its scales' buffer
         uint32_t ps = 0, pk = 0, pstage = 0, pgrp = 2, grp = 2, stage = 0;
         bool pending = false;
-        auto ahead = [&] {
+        // aims at the step that is loaded next; its scales are loaded before it, so
+        // that the wait for it covers them
+        auto aim_next = [&] {
             if (pk == 0) aim(min(ps, slots - 1));
-            if (pk % kGroup == 0) {  // (before the step's own loads, whose wait then covers them)
+            if (pk % kGroup == 0) {
                 load_scales(min(ps, slots - 1), pk);
                 pending = true;
                 pgrp = pgrp == 2 ? 0 : pgrp + 1;
             }
             __builtin_amdgcn_sched_barrier(0);
-            load(pstage, pk);
+        };
+        auto loaded = [&] {
             pstage = pstage == kStages - 1 ? 0 : pstage + 1;
             if (++pk == nk) pk = 0, ps++;
+        };
+        auto ahead = [&] {
+            aim_next();
+#pragma unroll
+            for (int i = 0; i < kLoads; i++) load(i, pstage, pk);
+            loaded();
         };
         auto store_scales = [&] {
             if (pending) keep_scales(pgrp);
@@ -675,8 +687,9 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
                 __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4) | (0 << 8));
                 __builtin_amdgcn_s_barrier();
                 __builtin_amdgcn_sched_barrier(0);
-                ahead();
-                compute(acc, stage, kb, grp);
+                aim_next();
+                compute(acc, stage, kb, grp, pstage, pk);
+                loaded();
                 stage = stage == kStages - 1 ? 0 : stage + 1;
             }
             const Tile t = lds.slot[s];
