@@ -484,15 +484,16 @@ constexpr int kGroup = 8, kStages = 3, kTileWaves = 8, kTileRows = 128, kTileCol
 struct TileLds {
     uint8_t x[kStages][kTileRows * 128];
     uint8_t w[kStages][kTileCols * 128];
-    uint16_t sx[3][kGroup][kTileRows];  // scales of kGroup steps: the current ones, the next, and those being stored
-    float sw[3][2][kGroup];
+    uint16_t sx[4][kGroup][kTileRows];  // scales of kGroup steps: of the four steps from the current one on
+    float sw[4][2][kGroup];
     uint32_t tops[4 * kTileRows];
     uint32_t map[kSlots][kTileRows];  // SWIGLU: input row of each position; else its output row; 0xffffffff: none
     Tile slot[kSlots];
     uint32_t scan[kTileWaves];
 };
 
-template <int MODE>
+// TAIL: `in` is no multiple of 128
+template <int MODE, bool TAIL>
 __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
     constexpr bool kF16 = MODE == F32OUT;
     constexpr int NX = 2, NW = 4;     // DMA instructions of a wave and step: token rows, weight rows
@@ -500,7 +501,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
     __shared__ __attribute__((aligned(16))) TileLds lds;
     const uint32_t tid = threadIdx.x, lane = tid & 63, c = lane & 15, q = lane >> 4;
     const uint32_t wv = __builtin_amdgcn_readfirstlane(tid >> 6), wg = wv >> 1, tg = wv & 1;
-    const uint32_t nk = a.kb, tail = a.in % 128, ob = (a.out + 127) / 128;
+    const uint32_t nk = a.kb, tail = TAIL ? a.in % 128 : 0, ob = (a.out + 127) / 128;
     const __amdgpu_buffer_rsrc_t rx = buffer_rsrc(a.x, (uint32_t)((uint64_t)a.xrows * a.in));
     const uint32_t wbytes = (uint32_t)((uint64_t)a.out * a.in);
     // DMA: instruction i of wave wv fills LDS rows 8 (8 i + wv) .. + 7; lane l
@@ -533,10 +534,10 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
     };
     // columns past `in` in the last step: a chunk is replaced by its row's first of
     // the block, and the weights' codes are zeroed when they are used
-    const uint32_t back = tail && dchunk >= tail ? dchunk : 0;
+    const uint32_t back = TAIL && dchunk >= tail ? dchunk : 0;
     // one of the kLoads instructions of block kb into `stage`
     auto load = [&](int i, uint32_t stage, uint32_t kb) {
-        const uint32_t b = kb + 1 == nk ? back : 0;
+        const uint32_t b = TAIL && kb + 1 == nk ? back : 0;
         if (i < NX)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lds_ptr)(lds.x[stage] + (64 * i + 8 * wv) * 128), 16,
                                                      xoff[i < NX ? i : 0] - b, kb * 128, 0, 0);
@@ -571,19 +572,30 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
     auto codes = [&](const uint8_t *rows) {
         return Codes{*reinterpret_cast<const u32x4q *>(rows + lo), *reinterpret_cast<const u32x4q *>(rows + hi)};
     };
-    // a step over the wave's first NS token tiles (tile i: rows 32 i + 16 tg on);
-    // the DMA of block lkb into lstage is issued between the products (in one
-    // go it held the waves up until the memory pipe had taken all of it)
-    auto compute = [&](auto &acc, uint32_t stage, uint32_t kb, uint32_t grp, uint32_t lstage, uint32_t lkb) {
-        constexpr int NS = sizeof(acc[0]) / sizeof(acc[0][0]);
-        const uint8_t *xr = xbase + stage * (kTileRows * 128), *wr = wbase + stage * (kTileCols * 128);
-        const float sw = lds.sw[grp][MODE == SWIGLU ? 0 : wg >> 1][kb % kGroup];
-        const float sw2 = MODE == SWIGLU ? lds.sw[grp][1][kb % kGroup] : sw;
-        const uint16_t *sx = lds.sx[grp][kb % kGroup] + 16 * tg + c;
-        Codes wc[4];
+    auto weights = [&](uint32_t stage, int j) { return codes(wbase + stage * (kTileCols * 128) + j * 2048); };
+    auto tokens = [&](uint32_t stage, int i) { return codes(xbase + stage * (kTileRows * 128) + i * 4096); };
+    // What a wave holds of a step: its scales, raw, and its codes of NS token tiles
+    // (tile i: rows 32 i + 16 tg on) and four row tiles.
+    struct Scales {
+        float sw, sw2;
+        uint32_t sx[4];
+    };
+    auto scales = [&](auto &sc, uint32_t kb, uint32_t grp) {
+        sc.sw = lds.sw[grp][MODE == SWIGLU ? 0 : wg >> 1][kb % kGroup];
+        sc.sw2 = MODE == SWIGLU ? lds.sw[grp][1][kb % kGroup] : 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; j++) wc[j] = codes(wr + j * 2048);
-        if (tail && kb + 1 == nk) {
+        for (int i = 0; i < 4; i++) sc.sx[i] = lds.sx[grp][kb % kGroup][32 * i + 16 * tg + c];
+    };
+    // A step over codes wc, xc and scales sc; each is replaced by the next step's
+    // after its last use (from stage `next` and the scales' buffer ngrp), and
+    // `between`, after the first products, turns to the step to load,
+    // whose DMA is issued from there on (in one go it held the waves up until
+    // the memory pipe had taken all of it).  A block's sums join their running
+    // sums kLag products later.  In this order the matrix cores wait for neither.
+    auto compute = [&](auto &acc, Codes (&wc)[4], auto &xc, Scales &sc, uint32_t next, uint32_t kb, uint32_t ngrp,
+                       auto between) {
+        constexpr int NS = sizeof(acc[0]) / sizeof(acc[0][0]), kLag = 3;
+        if (TAIL && kb + 1 == nk) {
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 if (16 * q >= tail) wc[j].lo = u32x4q{0, 0, 0, 0};
@@ -591,30 +603,28 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
             }
         }
         const Operand<kF16> wo[4] = {Operand<kF16>(wc[0]), Operand<kF16>(wc[1]), Operand<kF16>(wc[2]), Operand<kF16>(wc[3])};
-        // A block's sums join their running sums kLag products later, and a
-        // token tile is read one tile ahead, in this order: the matrix cores
-        // then wait for neither.
-        constexpr int kLag = 3;
-        Codes xc[NS];
         float s1[NS], s2[NS];
+#pragma unroll
+        for (int i = 0; i < NS; i++) {
+            s1[i] = bf16_to_f32(sc.sx[i]) * sc.sw;
+            s2[i] = MODE == SWIGLU ? bf16_to_f32(sc.sx[i]) * sc.sw2 : 0.f;
+        }
         f32x4q d[4 * NS];
-        xc[0] = codes(xr);
-        s1[0] = bf16_to_f32(sx[0]);
+        uint32_t lstage = 0, lkb = 0;
 #pragma unroll
         for (int n = 0; n < 4 * NS + kLag; n++) {
             const int i = n / 4, j = n % 4;
             if (n < 4 * NS) {
-                if (j == 0) {
-                    if (i + 1 < NS) {
-                        xc[i + 1] = codes(xr + (i + 1) * 4096);
-                        s1[i + 1] = bf16_to_f32(sx[32 * (i + 1)]);
-                    }
-                    s2[i] = MODE == SWIGLU ? s1[i] * sw2 : 0.f;
-                    s1[i] *= sw;
-                }
                 d[n] = block_dot(wo[j], Operand<kF16>(xc[i]));
+                if (i == NS - 1) wc[j] = weights(next, j);
+                if (j == 3) xc[i] = tokens(next, i);
+                if (n == 1) between(lstage, lkb);
+                if (n == 3) scales(sc, kb + 1, ngrp);
+                if (n >= 3) {
+                    constexpr int R = 4 * NS - 3;
 #pragma unroll
-                for (int l = n * kLoads / (4 * NS); l < (n + 1) * kLoads / (4 * NS); l++) load(l, lstage, lkb);
+                    for (int l = (n - 3) * kLoads / R; l < (n - 2) * kLoads / R; l++) load(l, lstage, lkb);
+                }
             }
             if (n >= kLag) {
                 const int m = n - kLag;
@@ -642,7 +652,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
         __syncthreads();
         // the step that is loaded next: slot ps (past the last: the last again,
         // unused), block pk; the stage it goes to; its scales' buffer
-        uint32_t ps = 0, pk = 0, pstage = 0, pgrp = 2, grp = 2, stage = 0;
+        uint32_t ps = 0, pk = 0, pstage = 0, pgrp = 3, grp = 3, stage = 0;
         bool pending = false;
         // aims at the step that is loaded next; its scales are loaded before it, so
         // that the wait for it covers them
@@ -651,7 +661,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
             if (pk % kGroup == 0) {
                 load_scales(min(ps, slots - 1), pk);
                 pending = true;
-                pgrp = pgrp == 2 ? 0 : pgrp + 1;
+                pgrp = (pgrp + 1) % 4;
             }
             __builtin_amdgcn_sched_barrier(0);
         };
@@ -669,29 +679,46 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
             if (pending) keep_scales(pgrp);
             pending = false;
         };
+        // A step begins when the next one's rows are in LDS and this one's are read
+        // out: all but the loads of the step after the next have landed (gfx9
+        // encoding: vmcnt, then lgkmcnt 0), everyone's.
+        auto begin = [&] {
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_waitcnt(kLoads | (7 << 4) | (15 << 8));
+            store_scales();
+            __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4) | (0 << 8));
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+        };
         ahead();
         store_scales();
+        ahead();
+        begin();
         ahead();
         // slot s over the first NS token tiles of each wave
         auto item = [&](auto tiles, uint32_t s) {
             constexpr int NS = decltype(tiles)::value;
             f32x4q acc[4][NS] = {};
+            // (the item's first step is in LDS since the last item's last step began)
+            Codes wc[4], xc[NS];
+            Scales sc;
+#pragma unroll
+            for (int j = 0; j < 4; j++) wc[j] = weights(stage, j);
+#pragma unroll
+            for (int i = 0; i < NS; i++) xc[i] = tokens(stage, i);
+            grp = (grp + 1) % 4;
+            scales(sc, 0, grp);
             for (uint32_t kb = 0; kb < nk; kb++) {
-                if (kb % kGroup == 0) grp = grp == 2 ? 0 : grp + 1;
-                // a step begins when its rows are in LDS: all but the loads of the step
-                // after it have landed (gfx9 encoding: vmcnt, then lgkmcnt 0 for the
-                // scales), everyone's, and nobody reads the buffer that is filled next
-                __builtin_amdgcn_sched_barrier(0);
-                __builtin_amdgcn_s_waitcnt(kLoads | (7 << 4) | (15 << 8));
-                store_scales();
-                __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4) | (0 << 8));
-                __builtin_amdgcn_s_barrier();
-                __builtin_amdgcn_sched_barrier(0);
-                aim_next();
-                compute(acc, stage, kb, grp, pstage, pk);
-                loaded();
                 stage = stage == kStages - 1 ? 0 : stage + 1;
+                begin();
+                if (kb % kGroup == kGroup - 1) grp = (grp + 1) % 4;  // the next step's
+                compute(acc, wc, xc, sc, stage, kb, grp, [&](uint32_t &lstage, uint32_t &lkb) {
+                    aim_next();
+                    lstage = pstage, lkb = pk;
+                    loaded();
+                });
             }
+            if (nk % kGroup == 0) grp = (grp + 3) % 4;  // (the last step looked past the item)
             const Tile t = lds.slot[s];
             const uint32_t ct = __builtin_amdgcn_readfirstlane(t.ct);
             uint32_t to[NS];
@@ -713,8 +740,8 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
             else if (live > 32) item(std::integral_constant<int, 2>{}, s);
             else item(std::integral_constant<int, 1>{}, s);
         }
-        if (slots < kSlots) return;
         __builtin_amdgcn_s_waitcnt(0);  // the loads past the last item have landed
+        if (slots < kSlots) return;
         __syncthreads();
     }
 }
@@ -821,7 +848,7 @@ static hipError_t launch_q8(Prof *p, hipStream_t s, const char *name, q8::Args a
                                  (const float *)scratch);
         }
     }
-    const Form f = tiled ? Form{MODE == SWIGLU ? 128u : 256u, 512, tile_kernel<MODE>}
+    const Form f = tiled ? Form{MODE == SWIGLU ? 128u : 256u, 512, a.in % 128 ? tile_kernel<MODE, true> : tile_kernel<MODE, false>}
                    : two ? stream_form<MODE, 2>(a.out, a.kb, tiles)
                          : stream_form<MODE, 1>(a.out, a.kb, tiles);
     return launch_form(p, s, name, f, tiles, a, tiled ? kCus : 0x7fffffff);
