@@ -590,10 +590,10 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
     // after its last use (from stage `next` and the scales' buffer ngrp), and
     // `between`, after the first products, turns to the step to load,
     // whose DMA is issued from there on (in one go it held the waves up until
-    // the memory pipe had taken all of it).  A block's sums join their running
+    // the memory pipe had taken all of it; none without `loads`).  A block's sums join their running
     // sums kLag products later.  In this order the matrix cores wait for neither.
     auto compute = [&](auto &acc, Codes (&wc)[4], auto &xc, Scales &sc, uint32_t next, uint32_t kb, uint32_t ngrp,
-                       auto between) {
+                       bool loads, auto between) {
         constexpr int NS = sizeof(acc[0]) / sizeof(acc[0][0]), kLag = 3;
         if (TAIL && kb + 1 == nk) {
 #pragma unroll
@@ -618,12 +618,13 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
                 d[n] = block_dot(wo[j], Operand<kF16>(xc[i]));
                 if (i == NS - 1) wc[j] = weights(next, j);
                 if (j == 3) xc[i] = tokens(next, i);
-                if (n == 1) between(lstage, lkb);
+                if (n == 1 && loads) between(lstage, lkb);
                 if (n == 3) scales(sc, kb + 1, ngrp);
                 if (n >= 3) {
                     constexpr int R = 4 * NS - 3;
 #pragma unroll
-                    for (int l = (n - 3) * kLoads / R; l < (n - 2) * kLoads / R; l++) load(l, lstage, lkb);
+                    for (int l = (n - 3) * kLoads / R; l < (n - 2) * kLoads / R; l++)
+                        if (loads) load(l, lstage, lkb);
                 }
             }
             if (n >= kLag) {
@@ -675,26 +676,124 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
             for (int i = 0; i < kLoads; i++) load(i, pstage, pk);
             loaded();
         };
+        auto barrier = [&] {  // of LDS traffic only: the loads stay in flight
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4) | (0 << 8));
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+        };
         auto store_scales = [&] {
             if (pending) keep_scales(pgrp);
             pending = false;
         };
         // A step begins when the next one's rows are in LDS and this one's are read
         // out: all but the loads of the step after the next have landed (gfx9
-        // encoding: vmcnt, then lgkmcnt 0), everyone's.
+        // encoding: vmcnt), everyone's.  Before an item's outputs all of them have
+        // (`landed`), so that its next step does not wait for the stores.
+        bool landed = false;
         auto begin = [&] {
             __builtin_amdgcn_sched_barrier(0);
-            __builtin_amdgcn_s_waitcnt(kLoads | (7 << 4) | (15 << 8));
+            if (!landed) __builtin_amdgcn_s_waitcnt(kLoads | (7 << 4) | (15 << 8));
+            landed = false;
             store_scales();
-            __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4) | (0 << 8));
-            __builtin_amdgcn_s_barrier();
-            __builtin_amdgcn_sched_barrier(0);
+            barrier();
         };
         ahead();
         store_scales();
         ahead();
         begin();
         ahead();
+        // An item's outputs, through LDS buffer `buf`: a lane's results are neighbours
+        // of one row, but neighbouring lanes hold different rows, and stores of that
+        // kind took 64 times a line each.  16-byte chunks are XOR-swizzled by their row.
+        auto outputs = [&](auto &acc, uint32_t s, uint32_t buf) {
+            constexpr int NS = sizeof(acc[0]) / sizeof(acc[0][0]);
+            const Tile t = lds.slot[s];
+            const uint32_t ct = __builtin_amdgcn_readfirstlane(t.ct);
+            if constexpr (MODE == SWIGLU) {
+                float act[NS][8];
+#pragma unroll
+                for (int i = 0; i < NS; i++) {
+                    uint32_t top = 0;
+#pragma unroll
+                    for (int r = 0; r < 8; r++) {
+                        act[i][r] = swiglu_of(acc[r / 4][i][r % 4], acc[2 + r / 4][i][r % 4]);
+                        // (out is a multiple of 16: all of the lane's columns count, or none)
+                        if (ct * 128 + wg * 32 + 8 * q < a.out) top = max(top, abs_word(act[i][r]));
+                    }
+                    top = max_xor32_u(max_xor16_u(top));
+                    if (q == 0) lds.tops[wg * kTileRows + 32 * i + 16 * tg + c] = top;
+                }
+                barrier();
+                auto scale_of = [&](uint32_t row) {
+                    const uint32_t *p = lds.tops + row;
+                    return q8_scale_bits(max(max(p[0], p[kTileRows]), max(p[2 * kTileRows], p[3 * kTileRows])));
+                };
+#pragma unroll
+                for (int i = 0; i < NS; i++) {
+                    const uint32_t row = 32 * i + 16 * tg + c, chunk = 2 * wg + (q >> 1);
+                    const float r = 1.0f / bf16_to_f32(scale_of(row));
+                    *reinterpret_cast<u32x2q *>(lds.x[buf] + row * 128 + ((chunk ^ (row & 7)) << 4) + 8 * (q & 1)) =
+                        u32x2q{q8_codes4(act[i][0], act[i][1], act[i][2], act[i][3], r),
+                               q8_codes4(act[i][4], act[i][5], act[i][6], act[i][7], r)};
+                }
+                barrier();
+                if (tid < t.end - t.m0 && lds.map[s][tid] != 0xffffffffu)
+                    a.scales[(uint64_t)(t.m0 + tid) * ob + ct] = (uint16_t)scale_of(tid);
+#pragma unroll
+                for (int m = 0; m < 2; m++) {
+                    const uint32_t row = 16 * wv + 8 * m + lane / 8, chunk = lane % 8, col = ct * 128 + 16 * chunk;
+                    if (row < t.end - t.m0 && lds.map[s][row] != 0xffffffffu && col < a.out)
+                        *reinterpret_cast<u32x4q *>(a.codes + (uint64_t)(t.m0 + row) * a.out + col) =
+                            *reinterpret_cast<const u32x4q *>(lds.x[buf] + row * 128 + ((chunk ^ (row & 7)) << 4));
+                }
+            } else {
+                constexpr uint32_t B = MODE == F32OUT ? 4 : 2;              // bytes of a value
+                constexpr int P = MODE == F32OUT ? 1 : 2, C = 4 * B;        // token tiles and chunks of a row in 4 KiB
+                if (a.out % (16 / B) || (reinterpret_cast<uintptr_t>(a.y) & 15u)) {  // rows that start unaligned
+                    uint32_t to[NS];
+#pragma unroll
+                    for (int i = 0; i < NS; i++) to[i] = lds.map[s][32 * i + 16 * tg + c];
+                    store_rows<MODE, 4, NS>(a, acc, to, ct * 256 + wg * 64 + 16 * q);
+                    return;
+                }
+                uint8_t *const mine = lds.w[buf] + 4096 * wv;  // of this wave alone
+#pragma unroll
+                for (int h = 0; h < NS; h += P) {
+#pragma unroll
+                    for (int i = h; i < min(h + P, NS); i++) {
+                        uint8_t *const row = mine + (16 * (i - h) + c) * (16 * C);
+#pragma unroll
+                        for (int k = 0; k < C / 4; k++) {
+                            u32x4q v;
+                            if constexpr (MODE == F32OUT) {
+                                v = __builtin_bit_cast(u32x4q, acc[k][i]);
+                            } else {
+                                const f32x4q lo = acc[2 * k][i], hi = acc[2 * k + 1][i];
+                                v = u32x4q{bf16_pair(lo[0], lo[1]), bf16_pair(lo[2], lo[3]), bf16_pair(hi[0], hi[1]),
+                                           bf16_pair(hi[2], hi[3])};
+                            }
+                            *reinterpret_cast<u32x4q *>(row + (((C / 4 * q + k) ^ (c & (C - 1))) << 4)) = v;
+                        }
+                    }
+                    wave_lds_sync();
+#pragma unroll
+                    for (int m = 0; m < 16 * P * C / 64; m++) {
+                        const uint32_t r = (64 * m + lane) / C, chunk = lane % C;  // row of the staged ones
+                        const int i = h + m * (64 / C) / 16;
+                        const uint32_t col = ct * 256 + wg * 64 + chunk * (16 / B);
+                        if (i >= NS) continue;
+                        const u32x4q v = *reinterpret_cast<const u32x4q *>(mine + r * (16 * C) + ((chunk ^ (r & (C - 1))) << 4));
+                        const uint32_t to = lds.map[s][32 * i + 16 * tg + r % 16];
+                        if (to != 0xffffffffu && col < a.out)
+                            *reinterpret_cast<u32x4q *>(static_cast<uint8_t *>(a.y) + ((uint64_t)to * a.out + col) * B) = v;
+                    }
+                    wave_lds_sync();
+                }
+            }
+        };
         // slot s over the first NS token tiles of each wave
         auto item = [&](auto tiles, uint32_t s) {
             constexpr int NS = decltype(tiles)::value;
@@ -708,29 +807,26 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
             for (int i = 0; i < NS; i++) xc[i] = tokens(stage, i);
             grp = (grp + 1) % 4;
             scales(sc, 0, grp);
-            for (uint32_t kb = 0; kb < nk; kb++) {
+            auto step = [&](uint32_t kb, bool loads) {
                 stage = stage == kStages - 1 ? 0 : stage + 1;
                 begin();
                 if (kb % kGroup == kGroup - 1) grp = (grp + 1) % 4;  // the next step's
-                compute(acc, wc, xc, sc, stage, kb, grp, [&](uint32_t &lstage, uint32_t &lkb) {
+                compute(acc, wc, xc, sc, stage, kb, grp, loads, [&](uint32_t &lstage, uint32_t &lkb) {
                     aim_next();
                     lstage = pstage, lkb = pk;
                     loaded();
                 });
-            }
+            };
+            for (uint32_t kb = 0; kb + 1 < nk; kb++) step(kb, true);
+            // the buffer that the last step's loads would fill serves the outputs
+            // first: they leave through it in whole lines
+            step(nk - 1, false);
             if (nk % kGroup == 0) grp = (grp + 3) % 4;  // (the last step looked past the item)
-            const Tile t = lds.slot[s];
-            const uint32_t ct = __builtin_amdgcn_readfirstlane(t.ct);
-            uint32_t to[NS];
-#pragma unroll
-            for (int i = 0; i < NS; i++) {
-                const uint32_t r = 32 * i + 16 * tg + c, m = lds.map[s][r];
-                to[i] = MODE == SWIGLU && m != 0xffffffffu ? t.m0 + r : m;
-            }
-            if constexpr (MODE == SWIGLU)
-                store_swiglu<4, NS, kTileRows, 4, 32>(a, acc, to, ct * 128 + wg * 32 + 8 * q, ct, wg, 16 * tg, lds.tops);
-            else
-                store_rows<MODE, 4, NS>(a, acc, to, ct * 256 + wg * 64 + 16 * q);
+            __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));
+            landed = true;
+            outputs(acc, s, pstage);
+            barrier();
+            ahead();
         };
         for (uint32_t s = 0; s < slots; s++) {
             // (every wave takes the same way: the barriers are inside)
