@@ -243,10 +243,12 @@ __device__ __forceinline__ void store_rows(const Args &a, const f32x4q (&acc)[RT
     }
 }
 
-// silu(g) * u; the exponential and the reciprocal are within 2^-22 of theirs,
-// far below the 2^-4 of the 8-bit codes this becomes
+// silu(g) * u.  The rounding of log2(e) * g puts the exponential off by up to
+// |g| 2^-23 of it: 2^-16 where silu(g) is not yet 0, far below the 2^-4 of the 8-bit
+// codes this becomes.
 __device__ __forceinline__ float swiglu_of(float g, float u) {
-    return g * __builtin_amdgcn_rcpf(1.0f + exp_fast(-g)) * u;
+    constexpr float kLog2e = 1.44269504f;
+    return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * g)) * u;
 }
 
 // SWIGLU: row tiles 0 .. RT/2 - 1 of acc are gate rows, the rest their up rows.
@@ -282,7 +284,7 @@ __device__ __forceinline__ void store_swiglu(const Args &a, const f32x4q (&acc)[
         for (int v = 1; v < NW; v++) top = max(top, tops[v * BM + at]);
         const uint32_t sb = q8_scale_bits(top);
         if (to[i] == 0xffffffffu) continue;
-        const float r = 1.0f / bf16_to_f32(sb);
+        const float r = q8_inverse(sb);
         if (cols_in) {
             uint32_t *o = reinterpret_cast<uint32_t *>(a.codes + (uint64_t)to[i] * a.out + col);
             if constexpr (V == 8)
@@ -720,9 +722,10 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
 #pragma unroll
                     for (int r = 0; r < 8; r++) {
                         act[i][r] = swiglu_of(acc[r / 4][i][r % 4], acc[2 + r / 4][i][r % 4]);
-                        // (out is a multiple of 16: all of the lane's columns count, or none)
-                        if (ct * 128 + wg * 32 + 8 * q < a.out) top = max(top, abs_word(act[i][r]));
+                        top = max(top, abs_word(act[i][r]));
                     }
+                    // (out is a multiple of 16: all of the lane's columns count, or none)
+                    if (ct * 128 + wg * 32 + 8 * q >= a.out) top = 0;
                     top = max_xor32_u(max_xor16_u(top));
                     if (q == 0) lds.tops[wg * kTileRows + 32 * i + 16 * tg + c] = top;
                 }
@@ -734,7 +737,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
 #pragma unroll
                 for (int i = 0; i < NS; i++) {
                     const uint32_t row = 32 * i + 16 * tg + c, chunk = 2 * wg + (q >> 1);
-                    const float r = 1.0f / bf16_to_f32(scale_of(row));
+                    const float r = q8_inverse(scale_of(row));
                     *reinterpret_cast<u32x2q *>(lds.x[buf] + row * 128 + ((chunk ^ (row & 7)) << 4) + 8 * (q & 1)) =
                         u32x2q{q8_codes4(act[i][0], act[i][1], act[i][2], act[i][3], r),
                                q8_codes4(act[i][4], act[i][5], act[i][6], act[i][7], r)};
@@ -870,7 +873,7 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(Args a, const float 
         for (int j = 0; j < 8; j++) top = max(top, abs_word(v[j]));
         const uint32_t sb = q8_scale_bits(row16_max(top));
         if (!live) continue;
-        const float r = 1.0f / bf16_to_f32(sb);
+        const float r = q8_inverse(sb);
         *reinterpret_cast<u32x2q *>(a.codes + (uint64_t)p * a.out + i) =
             u32x2q{q8_codes4(v[0], v[1], v[2], v[3], r), q8_codes4(v[4], v[5], v[6], v[7], r)};
         if ((tid & 15) == 0) a.scales[(uint64_t)p * ob + i / 128] = (uint16_t)sb;

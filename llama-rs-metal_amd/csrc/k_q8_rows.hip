@@ -80,7 +80,7 @@ __global__ __launch_bounds__(kQ8NormThreads) void norm_q8_kernel(const float *x,
         }
         top = row16_max(top);
         const uint32_t sb = q8_scale_bits(top);
-        const float r = 1.0f / bf16_to_f32(sb);
+        const float r = q8_inverse(sb);
         if (!live) return;
         if (y) store(y, i, o);
         *reinterpret_cast<u32x2q *>(codes + base + i) =

@@ -21,8 +21,7 @@ __device__ __forceinline__ uint32_t abs_word(float x) { return __float_as_uint(x
 
 // F32 to bf16 bits, nearest even; NaN stays NaN.
 __device__ __forceinline__ uint32_t bf16_bits(float x) {
-    const uint32_t b = __float_as_uint(x);
-    return abs_word(x) > 0x7f800000u ? (b >> 16) | 0x40u : (b + 0x7fffu + ((b >> 16) & 1u)) >> 16;
+    return __builtin_bit_cast(uint16_t, static_cast<__bf16>(x));
 }
 
 // The maximum over each aligned row of 16 lanes, all of which are active.
@@ -35,11 +34,16 @@ __device__ __forceinline__ uint32_t row16_max(uint32_t v) {
 
 // The stored scale of 128 values whose largest magnitude (abs_word) is `top`.
 // A group that holds an infinity or a NaN gets a scale of infinity or NaN, so
-// each of its values reads back as NaN (0 * inf, NaN * inf).
+// each of its values reads back as NaN (0 * inf, NaN * inf).  The quotient of the
+// product with 1/448 and one correction is the division's for every finite `top`
+// whose quotient is kQ8Least or more.
 __device__ __forceinline__ uint32_t q8_scale_bits(uint32_t top) {
-    const float s = __uint_as_float(top) / kQ8Top;
-    return bf16_bits(s < kQ8Least ? kQ8Least : s);
+    const float x = __uint_as_float(top), q = x * (1.0f / kQ8Top);
+    const float s = fmaf(fmaf(-q, kQ8Top, x), 1.0f / kQ8Top, q);
+    return bf16_bits(x < kQ8Least * kQ8Top ? kQ8Least : top >= 0x7f800000u ? x : s);
 }
+// 1 / scale, within 2^-23 of it (a scale is at least 2^-126)
+__device__ __forceinline__ float q8_inverse(uint32_t sb) { return __builtin_amdgcn_rcpf(bf16_to_f32(sb)); }
 // Four values as e4m3 codes (nearest even; r: 1 / scale).  |v| * r is at most
 // 448 * (1 + 2^-8), which rounds to 448.
 __device__ __forceinline__ uint32_t q8_codes4(float a, float b, float c, float d, float r) {
