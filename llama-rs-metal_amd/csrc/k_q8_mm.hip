@@ -57,14 +57,17 @@ struct Args {
 // segment, experts ascending) times a column tile.  Workgroup b runs on XCD
 // b % 8; the items are split into eight contiguous ranges, one per XCD, so the
 // tiles that share an expert's weights and a run's rows meet in one L2; the
-// blocks of an XCD take its range's items in turn.  Every thread of the block
-// calls it; slots `from` and on of the block are written to out[0 .. n), at most
+// blocks of an XCD take its range's items in turn.  Segments of many tiles both
+// ways go by panels of kPanel column tiles, so that the 32 items an XCD has in
+// hand read 4 tiles of weights and 8 of tokens rather than all weights (4096 rows,
+// 4096 to 12288 columns: 200 us; 205 with panels of 8, 224 of 1, 247 of all).
+// Every thread of the block calls it; slots `from` and on of the block are written to out[0 .. n), at most
 // kMax; n is returned.  Offsets past P count as P and a segment that ends before
 // it starts is empty.
 struct Tile {
     uint32_t e, m0, end, ct;
 };
-constexpr uint32_t kXcds = 8;
+constexpr uint32_t kXcds = 8, kPanel = 4;
 template <int BM, int NW>
 __device__ __forceinline__ uint32_t find_items(const Args &a, uint32_t from, uint32_t kMax, Tile *out, uint32_t *lds /* NW */) {
     const uint32_t tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
@@ -98,30 +101,33 @@ __device__ __forceinline__ uint32_t find_items(const Args &a, uint32_t from, uin
             total += lds[v];
         }
     }
-    const uint64_t items = (uint64_t)total * a.col_tiles, range = (items + kXcds - 1) / kXcds;
-    const uint64_t lo_item = blockIdx.x % kXcds * range, hi_item = min(items, lo_item + range);
+    // (fewer than 2^31 items: the launch checks it)
+    const uint32_t items = total * a.col_tiles, range = (items + kXcds - 1) / kXcds;
+    const uint32_t lo_item = blockIdx.x % kXcds * range, hi_item = min(items, lo_item + range);
     const uint32_t turn = gridDim.x / kXcds;
-    const uint64_t first = lo_item + blockIdx.x / kXcds + (uint64_t)from * turn;
+    const uint32_t first = lo_item + blockIdx.x / kXcds + from * turn;
     if (first >= hi_item) return 0;
-    const uint32_t n = (uint32_t)min((uint64_t)kMax, (hi_item - first + turn - 1) / turn);
+    const uint32_t n = min(kMax, (hi_item - first + turn - 1) / turn);
+    // item `i` of a segment of k tiles
+    auto put = [&](uint32_t s, uint32_t e, uint32_t lo, uint32_t hi, uint32_t k, uint32_t i) {
+        const uint32_t panel = k < 2 * kPanel || a.col_tiles <= 2 * kPanel ? a.col_tiles : kPanel;
+        const uint32_t ct = i / (k * panel) * panel;
+        const uint32_t wide = min(panel, a.col_tiles - ct), at = i - k * ct;
+        const uint32_t m0 = lo + at / wide * BM;
+        out[s] = Tile{e, m0, hi - m0 < BM ? hi : m0 + BM, ct + at % wide};
+    };
     if (!a.offsets) {
-        if (tid < n) {
-            const uint64_t item = first + (uint64_t)tid * turn;
-            const uint32_t tile = (uint32_t)(item / a.col_tiles), m0 = tile * BM;
-            out[tid] = Tile{0, m0, min(a.P, m0 + BM), (uint32_t)(item - (uint64_t)tile * a.col_tiles)};
-        }
+        if (tid < n) put(tid, 0, 0, a.P, total, first + tid * turn);
     } else {
         for (uint32_t s = 0; s < n; s++) {
-            const uint64_t item = first + (uint64_t)s * turn;
-            const uint32_t tile = (uint32_t)(item / a.col_tiles);
+            const uint32_t item = first + s * turn, tile = item / a.col_tiles;
             if (tile < before || tile >= before + mine) continue;
             uint32_t at = before;
             for (uint32_t i = 0; i < per && e0 + i < a.experts; i++) {
                 uint32_t lo, k;
                 const uint32_t hi = seg(e0 + i, lo, k);
                 if (tile - at < k) {
-                    const uint32_t m0 = lo + (tile - at) * BM;
-                    out[s] = Tile{e0 + i, m0, min(hi, m0 + BM), (uint32_t)(item - (uint64_t)tile * a.col_tiles)};
+                    put(s, e0 + i, lo, hi, k, item - at * a.col_tiles);
                     break;
                 }
                 at += k;
@@ -909,11 +915,11 @@ static Form stream_form(uint32_t out, uint32_t kb, uint64_t tiles) {
 }
 
 static hipError_t launch_form(Prof *p, hipStream_t s, const char *name, const Form &f, uint64_t tiles, q8::Args a,
-                              uint64_t most_blocks = 0x7fffffff) {
+                              uint64_t most_blocks = 0x7ffffff8) {
     a.col_tiles = (a.out + f.cols - 1) / f.cols;
     uint64_t blocks = (tiles * a.col_tiles + q8::kXcds - 1) / q8::kXcds * q8::kXcds;
-    if (blocks > most_blocks && most_blocks == q8::kCus) blocks = most_blocks;
-    if (blocks > 0x7fffffffull) return hipErrorInvalidConfiguration;
+    if (blocks > 0x7ffffff8ull) return hipErrorInvalidConfiguration;
+    if (blocks > most_blocks) blocks = most_blocks;
     return launch_kernel(p, name, f.kernel, dim3((uint32_t)blocks), dim3(f.threads), 0, s, a);
 }
 
@@ -950,7 +956,7 @@ static hipError_t launch_q8(Prof *p, hipStream_t s, const char *name, q8::Args a
     const Form f = tiled ? Form{MODE == SWIGLU ? 128u : 256u, 512, a.in % 128 ? tile_kernel<MODE, true> : tile_kernel<MODE, false>}
                    : two ? stream_form<MODE, 2>(a.out, a.kb, tiles)
                          : stream_form<MODE, 1>(a.out, a.kb, tiles);
-    return launch_form(p, s, name, f, tiles, a, tiled ? kCus : 0x7fffffff);
+    return launch_form(p, s, name, f, tiles, a, tiled ? kCus : 0x7ffffff8);
 }
 
 hipError_t launch_q8_rows(Prof *p, hipStream_t s, const char *name, const Q8Weight &w, const Q8Rows &x,
