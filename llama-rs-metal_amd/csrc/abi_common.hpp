@@ -69,7 +69,7 @@ struct moe_gpu {
     Prof prof;
 };
 
-constexpr uint64_t kQ8RowsLen = 1u << 18;  // its values
+constexpr uint64_t kQ8RowsLen = 2560 * 128;  // its values
 
 struct moe_graph {
     hipGraph_t graph = nullptr;

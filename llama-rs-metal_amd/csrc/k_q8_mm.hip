@@ -313,7 +313,6 @@ __device__ __forceinline__ void store_swiglu(const Args &a, const f32x4q (&acc)[
 // leaves the codes in flight.
 constexpr uint32_t kChunk = 64;
 constexpr uint64_t kCus = 256;
-constexpr uint64_t kSplitBlocks = 400;
 
 template <int MODE, int RT, int TT, int KS, int NW>
 struct StreamLds {
@@ -894,20 +893,23 @@ struct Form {
     void (*kernel)(q8::Args);
 };
 // Waves of 16 rows, split along the columns until the launch has 1024 of them
-// or each two blocks; 32 rows where there are plenty.
+// or each two blocks; 32 rows where there are plenty, or few columns to load ahead
+// (16 experts of 768 columns to 2048, 128 rows: 7.8 us, with 16 rows 10.2; 512
+// experts of 512, 10 rows: 5.3, 7.7).
 template <int MODE, int TT>
 static Form stream_form(uint32_t out, uint32_t kb, uint64_t tiles) {
     using namespace q8;
     const uint64_t waves = (uint64_t)((out + 15) / 16) * tiles;
     if constexpr (MODE == SWIGLU) {
-        return Form{128, 512, stream_kernel<SWIGLU, 2, TT, 1, 8, TT == 1 ? 2 : 3, TT == 1 ? 4 : 2>};
+        return Form{128, 512, stream_kernel<SWIGLU, 2, 1, 1, 8, 2, 4>};
     } else if constexpr (MODE == ACT) {
         if (waves >= 1024 || kb < 4) return Form{64, 256, stream_kernel<ACT, 2, TT, 1, 4, 4, 2>};
         if (waves >= 512 || kb < 8) return Form{32, 256, stream_kernel<ACT, 2, TT, 2, 4, 4, 2>};
         return Form{16, 256, stream_kernel<ACT, 2, TT, 4, 4, 4, 2>};
     } else {
-        if (waves >= 4096) return Form{128, 256, stream_kernel<MODE, 2, TT, 1, 4, TT == 1 ? 2 : 3, TT == 1 ? 4 : 2>};
-        if (waves >= 1024 || kb < 4) return Form{64, 256, stream_kernel<MODE, 1, TT, 1, 4, TT == 1 ? 8 : 4, 2>};
+        if (waves >= 2048 || (TT == 1 && waves >= 1024 && kb < 8))
+            return Form{128, 256, stream_kernel<MODE, 2, TT, 1, 4, TT == 1 ? 2 : 3, TT == 1 ? 4 : 2>};
+        if (waves >= 1024 || kb < 4) return Form{64, 256, stream_kernel<MODE, 1, TT, 1, 4, TT == 1 && MODE == BF16OUT ? 8 : 4, 2>};
         if (waves >= 512 || kb < 8) return Form{32, 256, stream_kernel<MODE, 1, TT, 2, 4, 4, 2>};
         if (waves >= 256 || kb < 16) return Form{16, 256, stream_kernel<MODE, 1, TT, 4, 4, 4, 2>};
         return Form{16, 512, stream_kernel<MODE, 1, TT, 8, 8, 4, 2>};
@@ -930,20 +932,36 @@ static hipError_t launch_q8(Prof *p, hipStream_t s, const char *name, q8::Args a
     using namespace q8;
     a.kb = (a.in + 127) / 128;
     const uint32_t experts = a.offsets ? a.experts : 1;
+    const uint64_t live = experts < a.P ? experts : a.P, cols = MODE == SWIGLU ? 128 : 256, ct = (a.out + cols - 1) / cols;
     // every non-empty segment may end in a partial tile
-    auto max_tiles = [&](uint32_t bm) {
-        return a.P / bm + (a.offsets ? (uint64_t)(experts < a.P ? experts : a.P) : (uint64_t)(a.P % bm != 0));
-    };
-    // DMA offsets are 32-bit
-    const bool tiled = a.P >= (a.offsets ? 8ull : 33ull) * experts && (uint64_t)a.xrows * a.in < 0xffffffffull && (uint64_t)a.out * a.in < 0xffffffffull;
-    const bool two = !a.offsets && a.P > 16;
-    const uint32_t bm = tiled ? 128 : two ? 32 : 16;
-    const uint64_t tiles = max_tiles(bm);
+    auto max_tiles = [&](uint32_t bm) { return a.P / bm + (a.offsets ? live : (uint64_t)(a.P % bm != 0)); };
+    // Tiles of 128 rows need CUs to work on them: enough items, or enough rows
+    // (2048 columns, microseconds of tiles against the best stream form):
+    //   SwiGLU  512 outputs, 1 expert, 512 rows (16 items): 19.0, 16.1;  4 experts, 1024 rows (32): 19.5, 26.2
+    //           768 outputs, 16 experts, 64 rows (96 items): 15.7, 17.8;  2048 rows: 21.7, 73.6
+    //   bf16    4096 outputs, 128 rows (16 items): 16.8, 13.6;  256 rows (32): 17.3, 24.3
+    //           16384 outputs, 32 rows (64 items): 14.2, 13.8;  48 rows: 14.2, 24.4
+    //   F32     4096 outputs, 256 rows (32 items): 31.6, 25.4;  512 rows (64): 34.0, 38.3
+    // and an expert's rows to be worth its steps (768 columns to 2048, 64 experts):
+    //   bf16    512 rows: 21.6, 18.9;  1024: 21.9, 24.9      F32  512 rows: 24.4, 19.9;  1024: 24.8, 26.1
+    // SwiGLU's steps are worth it from the first row on (2048 to 512, 512 experts: 40 rows 17.5, 21.8;
+    // 640: 131, 131).  DMA offsets are 32-bit.
+    constexpr uint64_t kRows = MODE == SWIGLU ? 0 : MODE == F32OUT ? 16 : 12;
+    const bool fills = ct * a.P >= (MODE == F32OUT ? 5120 : 2560) || (MODE != F32OUT && ct * live >= 80);
+    const bool tiled = fills && a.P >= kRows * experts && (uint64_t)a.xrows * a.in < 0xffffffffull &&
+                       (uint64_t)a.out * a.in < 0xffffffffull;
+    // Two token tiles a wave read the weights half as often, where that leaves 256
+    // waves (24 rows, 2048 columns to 4096: 5.1 us against 6.2; 4096 to 2048: 7.6 against 6.3)
+    const bool two = a.P > 16ull * experts && (uint64_t)((a.out + 15) / 16) * ((a.P + 15) / 16) >= 512;
+    if (tiled)
+        return launch_form(p, s, name, Form{(uint32_t)cols, 512, a.in % 128 ? tile_kernel<MODE, true> : tile_kernel<MODE, false>},
+                           max_tiles(128), a, kCus);
+    const uint64_t tiles = max_tiles(two ? 32 : 16);
     if constexpr (MODE == SWIGLU) {
-        // Blocks of 128 outputs (512 KiB of weights at 2048 columns) leave most
-        // of the CUs idle when there are few: then blocks of 16 to 64 outputs
-        // write F32 rows, and a second launch quantises them.
-        if (!tiled && tiles * ((a.out + 127) / 128) <= kSplitBlocks && (uint64_t)a.P * a.out <= scratch_len) {
+        // A scale needs 128 outputs: blocks that hold them (512 KiB of weights at
+        // 2048 columns) are few, so blocks of 16 to 64 write F32 rows and a second
+        // launch quantises them.  (What does not fit has 2^32 bytes of rows or weights.)
+        if ((uint64_t)a.P * a.out <= scratch_len) {
             Args b = a;
             b.y = scratch;
             const hipError_t e = launch_form(p, s, name, two ? stream_form<ACT, 2>(a.out, a.kb, tiles)
@@ -952,11 +970,11 @@ static hipError_t launch_q8(Prof *p, hipStream_t s, const char *name, q8::Args a
             return launch_kernel(p, "quantize_q8", quantize_kernel, dim3(a.P), dim3(kThreads), 0, s, a,
                                  (const float *)scratch);
         }
+        return launch_form(p, s, name, stream_form<SWIGLU, 1>(a.out, a.kb, max_tiles(16)), max_tiles(16), a);
+    } else {
+        return launch_form(p, s, name, two ? stream_form<MODE, 2>(a.out, a.kb, tiles) : stream_form<MODE, 1>(a.out, a.kb, tiles),
+                           tiles, a);
     }
-    const Form f = tiled ? Form{MODE == SWIGLU ? 128u : 256u, 512, a.in % 128 ? tile_kernel<MODE, true> : tile_kernel<MODE, false>}
-                   : two ? stream_form<MODE, 2>(a.out, a.kb, tiles)
-                         : stream_form<MODE, 1>(a.out, a.kb, tiles);
-    return launch_form(p, s, name, f, tiles, a, tiled ? kCus : 0x7ffffff8);
 }
 
 hipError_t launch_q8_rows(Prof *p, hipStream_t s, const char *name, const Q8Weight &w, const Q8Rows &x,
