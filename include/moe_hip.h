@@ -357,12 +357,13 @@ moe_status moe_matmul_q8(moe_gpu *gpu, const moe_weight *w, moe_rows8 x, moe_buf
  * t*k + i.  q[p] = silu(x_t . G_e) * (x_t . U_e) in 8 bits, in position order;
  * q.rows = x.rows * k positions.  perm empty: position p reads row p (k = 1).
  * Ends past q.rows count as q.rows; positions of no segment, and positions
- * whose perm names no row, are left as they were. */
+ * whose perm names no row, are left as they were.  Segments do not overlap. */
 moe_status moe_expert_swiglu_q8(moe_gpu *gpu, const moe_weight *gate, const moe_weight *up,
                                 moe_rows8 x, moe_buffer offsets, moe_buffer perm, uint64_t k,
                                 moe_rows8 q);
 /* The same segments: y[perm[p]] = W_e x[p], one row of W's dims[1] values per
- * pair (perm empty: y[p]); x.rows positions. */
+ * pair (perm empty: y[p]); x.rows positions, whose perm entries are distinct (of
+ * a row named twice each value is that of one of its positions). */
 moe_status moe_expert_matmul_q8(moe_gpu *gpu, const moe_weight *w, moe_rows8 x,
                                 moe_buffer offsets, moe_buffer perm, moe_buffer y, uint32_t y_type);
 /* moe_mix for every token: y[t] = sum_i w[t*k + i] * x[t*k + i] (i ascending)

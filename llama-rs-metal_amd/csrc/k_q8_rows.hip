@@ -17,9 +17,10 @@ constexpr uint32_t kQ8NormThreads = 256, kQ8NormHold = 2;
 template <int T, bool VEC>
 __global__ __launch_bounds__(kQ8NormThreads) void norm_q8_kernel(const float *x, const float *resid, const void *w,
                                                                  float *sum, float *y, uint8_t *codes,
-                                                                 uint16_t *scales, uint32_t n, float eps) {
+                                                                 uint16_t *scales, uint32_t rows, uint32_t n, float eps) {
     __shared__ float part[kQ8NormThreads / 64];
-    const uint32_t row = blockIdx.x, tid = threadIdx.x, step = 8 * kQ8NormThreads;
+    const uint32_t row = blockIdx.y * gridDim.x + blockIdx.x, tid = threadIdx.x, step = 8 * kQ8NormThreads;
+    if (row >= rows) return;
     const uint64_t base = (uint64_t)row * n;
     auto load = [&](const float *p, uint32_t i, float *v) {
         if constexpr (VEC) {
@@ -121,8 +122,10 @@ hipError_t launch_norm_q8(Prof *p, hipStream_t s, const float *x, const float *r
                     : (wtype == 0   ? norm_q8_kernel<0, false>
                        : wtype == 1 ? norm_q8_kernel<1, false>
                                     : norm_q8_kernel<30, false>);
-    return launch_kernel(p, "norm_q8", kern, dim3(rows), dim3(kQ8NormThreads), 0, s, x, resid, w, sum, y, codes,
-                         scales, n, eps);
+    // a launch has fewer than 2^32 threads along x
+    const uint32_t wide = rows < (1u << 22) ? rows : 1u << 22;
+    return launch_kernel(p, "norm_q8", kern, dim3(wide, (rows + wide - 1) / wide), dim3(kQ8NormThreads), 0, s, x, resid,
+                         w, sum, y, codes, scales, rows, n, eps);
 }
 
 // y[t, i] = sum_k w[t, k] * x[t K + k, i] (k ascending) (+ resid[t, i])

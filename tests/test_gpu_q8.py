@@ -5,7 +5,7 @@ import pytest
 
 from helpers_q8 import (U, Weight8, bf16, check_quantized, cut_bound, decode, encode, f32_bound, nblocks, product,
                         quantize_rows, random_rows, rows_value, silu, spread)
-from hip_backend import BF16, E4M3, F16, F32, Batch, Buffer, GpuError, Rows8, ShapeError, Tensor
+from hip_backend import BF16, E4M3, F16, F32, Batch, Buffer, Gpu, Rows8, ShapeError, Tensor
 from hip_backend.api import MoeBufferC, MoeRegionC
 from hip_backend.synth import f32_to_bf16_bits
 
@@ -368,6 +368,225 @@ def test_expert_products_leave_other_rows(gpu, own):
         assert np.all(rows[~to] == 0x55555555) and not np.any((rows[to] == 0x55555555).all(1))
 
 
+# Segments of enough rows for tiles of 128 (8-bit outputs; bf16 from 12, F32 from 16 a segment).
+TILED = [
+    [2600], [33, 0, 64, 5, 1, 2500], [100, 31, 0, 129, 2400, 0, 96, 97], [260] * 10 + [4], [128] * 21,
+    [3, 0, 1, 0, 2, 43] * 17 + [500],
+]
+
+
+@pytest.mark.parametrize("lens", TILED, ids=lambda v: f"{len(v)}x{sum(v)}")
+@pytest.mark.parametrize("n_in,out", [(128, 64), (48, 300), (272, 130), (1040, 258)])
+@pytest.mark.parametrize("y_type,times", [(F32, 2), (BF16, 1)])
+def test_expert_matmul_q8_of_many_rows(gpu, own, lens, n_in, out, y_type, times):
+    rng = np.random.default_rng(sum(lens) + n_in)
+    lens = [n * times for n in lens]
+    E, P = len(lens), sum(lens)
+    w = Weight8(rng, E, out, n_in, [F32, BF16, F16][P % 3])
+    codes, bits = random_rows(rng, P, n_in)
+    offsets, perm = segments(rng, lens)
+    wd, x = own.weight(w.tensor()), own.rows8(P, n_in, codes, bits)
+    ob, pb = own.u32(offsets), own.u32(perm)
+    v = rows_value(codes, bits)
+    elems = P * out if y_type == F32 else P * out // 2
+    y = own.zeros(elems + 4, 0x7F7F7F7F)
+    seen = []
+    for at, p in ((0, pb), (0, None), (1, pb)):   # whole lines, no perm, rows that start unaligned
+        with gpu.batch() as b:
+            b.expert_matmul_q8(wd, x, ob, p, y.view(at, elems), y_type)
+        g = y.view(at, elems)
+        got = (gpu.read(g) if y_type == F32 else read_bf16(gpu, g)).reshape(P, out)
+        seen.append(got[perm] if p is not None else got)
+        assert np.all(gpu.read_u32(y)[elems + at:] == 0x7F7F7F7F)
+    assert np.array_equal(seen[0], seen[1]) and np.array_equal(seen[0], seen[2])
+    for e in range(E):
+        a, b_ = offsets[e], offsets[e + 1]
+        if b_ > a:
+            check_rows(seen[0][a:b_], *product(v[a:b_], w.value(e)), n_in, y_type == BF16)
+
+
+@pytest.mark.parametrize("lens", TILED, ids=lambda v: f"{len(v)}x{sum(v)}")
+@pytest.mark.parametrize("n_in,ff", [(128, 64), (48, 272), (272, 16), (1040, 144)])
+def test_expert_swiglu_q8_of_many_rows(gpu, own, lens, n_in, ff):
+    rng = np.random.default_rng(sum(lens) * 3 + n_in)
+    E, P = len(lens), sum(lens)
+    K = 2 if P % 2 == 0 else 1
+    st = [F32, BF16, F16][(P + ff // 16) % 3]
+    gate, up = Weight8(rng, E, ff, n_in, st), Weight8(rng, E, ff, n_in, st)
+    offsets, perm = segments(rng, lens)
+    codes, bits = random_rows(rng, P // K, n_in)
+    x, q = own.rows8(P // K, n_in, codes, bits), own.rows8(P, ff)
+    gd, ud, ob, pb = own.weight(gate.tensor()), own.weight(up.tensor()), own.u32(offsets), own.u32(perm)
+    with gpu.batch() as b:
+        b.expert_swiglu_q8(gd, ud, x, ob, pb, K, q)
+    got, gs = gpu.read_rows8(q)
+    v = rows_value(codes, bits)[perm // K]
+    for e in range(E):
+        a, b_ = offsets[e], offsets[e + 1]
+        if b_ > a:
+            check_quantized(got[a:b_], gs[a:b_], *swiglu64(v[a:b_], gate, up, e))
+
+
+@pytest.mark.parametrize("T,n_in,out", [(2600, 16, 64), (2561, 1040, 130), (900, 2064, 770), (300, 256, 2500),
+                                        (40, 128, 22000)])
+@pytest.mark.parametrize("y_type", [F32, BF16])
+def test_matmul_q8_of_many_rows(gpu, own, T, n_in, out, y_type):
+    T = T * 2 if y_type == F32 else T    # (tiles start at twice the rows)
+    rng = np.random.default_rng(T + n_in)
+    w = Weight8(rng, 1, out, n_in)
+    codes, bits = random_rows(rng, T, n_in)
+    wd, x = own.weight(w.tensor(dense=True)), own.rows8(T, n_in, codes, bits)
+    y = own.zeros(T * out if y_type == F32 else T * out // 2)
+    with gpu.batch() as b:
+        b.matmul_q8(wd, x, y, y_type)
+    got = (gpu.read(y) if y_type == F32 else read_bf16(gpu, y)).reshape(T, out)
+    check_rows(got, *product(rows_value(codes, bits), w.value()), n_in, y_type == BF16)
+
+
+def test_more_tiles_than_a_block_lists_at_once(gpu, own):
+    """256 blocks look their tiles up eight at a time: here each has nine or ten."""
+    rng = np.random.default_rng(31)
+    lens = [90000, 0, 7, 200, 179793]
+    E, P, n_in = len(lens), sum(lens), 16
+    w, w2 = Weight8(rng, E, 16, n_in), Weight8(rng, E, 16, n_in)
+    codes, bits = random_rows(rng, P, n_in)
+    offsets, perm = segments(rng, lens)
+    wd, ud, x, y = own.weight(w.tensor()), own.weight(w2.tensor()), own.rows8(P, n_in, codes, bits), own.zeros(P * 8)
+    ob, pb, q = own.u32(offsets), own.u32(perm), own.rows8(P, 16)
+    with gpu.batch() as b:
+        b.expert_matmul_q8(wd, x, ob, pb, y, BF16)
+        b.expert_swiglu_q8(wd, ud, x, ob, pb, 1, q)
+    got, (qc, qs) = read_bf16(gpu, y).reshape(P, 16)[perm], gpu.read_rows8(q)
+    v = rows_value(codes, bits)
+    for e in range(E):
+        a, b_ = offsets[e], offsets[e + 1]
+        if b_ > a:
+            check_rows(got[a:b_], *product(v[a:b_], w.value(e)), n_in, True)
+            check_quantized(qc[a:b_], qs[a:b_], *swiglu64(v[perm[a:b_]], w, w2, e))
+
+
+@pytest.mark.parametrize("T", [1, 5, 20, 40])
+@pytest.mark.parametrize("n_in", [8320, 16400])
+def test_long_rows(gpu, own, T, n_in):
+    """More blocks of 128 columns than the scales of one load."""
+    rng = np.random.default_rng(T + n_in)
+    w, w2 = Weight8(rng, 2, 48, n_in), Weight8(rng, 2, 48, n_in)
+    codes, bits = random_rows(rng, T, n_in)
+    wd, ud, x = own.weight(w.tensor()), own.weight(w2.tensor()), own.rows8(T, n_in, codes, bits)
+    ob, y, z, q = own.u32([0, T // 2, T]), own.zeros(T * 48), own.zeros(T * 24), own.rows8(T, 48)
+    with gpu.batch() as b:
+        b.expert_matmul_q8(wd, x, ob, None, y)
+        b.expert_matmul_q8(wd, x, ob, None, z, BF16)
+        b.expert_swiglu_q8(wd, ud, x, ob, None, 1, q)
+    v, (qc, qs) = rows_value(codes, bits), gpu.read_rows8(q)
+    for e, r in enumerate((slice(0, T // 2), slice(T // 2, T))):
+        if v[r].size:
+            check_rows(gpu.read(y).reshape(T, 48)[r], *product(v[r], w.value(e)), n_in, False)
+            check_rows(read_bf16(gpu, z).reshape(T, 48)[r], *product(v[r], w.value(e)), n_in, True)
+            check_quantized(qc[r], qs[r], *swiglu64(v[r], w, w2, e))
+
+
+@pytest.mark.parametrize("T", [3, 130, 3000])
+def test_shared_expert_and_rows_named_twice(gpu, own, T):
+    """One expert, no perm; then a perm that names rows more than once: each
+    position reads the row it names, and each value of a result row named twice
+    is that of one of its positions (which one may differ between the column
+    tiles, whose blocks write in no set order)."""
+    rng = np.random.default_rng(T)
+    w, w2, dn = Weight8(rng, 1, 144, 256), Weight8(rng, 1, 144, 256), Weight8(rng, 1, 256, 144)
+    codes, bits = random_rows(rng, T, 256)
+    wd, ud, x, q = own.weight(w.tensor()), own.weight(w2.tensor()), own.rows8(T, 256, codes, bits), own.rows8(T, 144)
+    dd, d3, y = own.weight(dn.tensor(dense=True)), own.weight(dn.tensor()), own.zeros(T * 128)
+    ob, twice = own.u32([0, T]), rng.integers(0, T, T)
+    pb, q2, y2 = own.u32(twice), own.rows8(T, 144), own.zeros(T * 128, 0x7FC07FC0)
+    with gpu.batch() as b:
+        b.expert_swiglu_q8(wd, ud, x, ob, None, 1, q)
+        b.matmul_q8(dd, q, y, BF16)
+        b.expert_swiglu_q8(wd, ud, x, ob, pb, 1, q2)
+        b.expert_matmul_q8(d3, q, ob, pb, y2, BF16)
+    qc, qs = gpu.read_rows8(q)
+    check_quantized(qc, qs, *swiglu64(rows_value(codes, bits), w, w2, 0))
+    got = read_bf16(gpu, y).reshape(T, 256)
+    check_rows(got, *product(rows_value(qc, qs), dn.value()), 144, True)
+    c2, s2 = gpu.read_rows8(q2)
+    assert np.array_equal(c2, qc[twice]) and np.array_equal(s2, qs[twice])
+    got2 = read_bf16(gpu, y2).reshape(T, 256)
+    for row in range(T):
+        at = np.flatnonzero(twice == row)
+        assert np.isnan(got2[row]).all() if at.size == 0 else (got2[row] == got[at]).any(0).all()
+
+
+def test_two_gpus_at_once(gpu, own):
+    """Batches of two engines on one device, both in flight: neither sees the
+    other's rows between the two launches of a small SwiGLU."""
+    rng = np.random.default_rng(17)
+    T, n_in, ff, E = 48, 512, 512, 4
+    w, w2 = Weight8(rng, E, ff, n_in), Weight8(rng, E, ff, n_in)
+    second = Gpu(0)
+    runs = []
+    for g in (gpu, second):
+        o = own if g is gpu else Owned(g)
+        codes, bits = random_rows(rng, T, n_in)
+        runs.append((g, o, o.weight(w.tensor()), o.weight(w2.tensor()), o.rows8(T, n_in, codes, bits),
+                     o.u32([0, 10, 10, 31, T]), o.rows8(T, ff), o.rows8(T, ff)))
+    for g, _, wd, ud, x, ob, q, _ in runs:
+        with g.batch() as b:
+            b.expert_swiglu_q8(wd, ud, x, ob, None, 1, q)
+    batches = [Batch(g) for g, *_ in runs]
+    for _ in range(50):
+        for b, (_, _, wd, ud, x, ob, _, r) in zip(batches, runs):
+            b.expert_swiglu_q8(wd, ud, x, ob, None, 1, r)
+    for b in batches:
+        b.finish()
+    for g, o, _, _, _, _, q, r in runs:
+        for i, j in zip(g.read_rows8(q), g.read_rows8(r)):
+            assert np.array_equal(i, j)
+    runs[1][1].release()
+
+
+def test_rows_past_four_gib(gpu, own):
+    """Row offsets that take more than 32 bits: the last rows of 4.3 GB of codes."""
+    rng = np.random.default_rng(8)
+    n_in, T, last = 8192, 524800, 96
+    w, w2 = Weight8(rng, 1, 16, n_in), Weight8(rng, 1, 16, n_in)
+    few, fb = random_rows(rng, 512, n_in)
+    codes, bits = np.tile(few, (T // 512, 1)), np.tile(fb, (T // 512, 1))
+    tail, tb = random_rows(rng, last, n_in)
+    codes[-last:], bits[-last:] = tail, tb
+    x, q, y, z = own.rows8(T, n_in, codes, bits), own.rows8(T, 16), own.zeros(T * 16), own.zeros(T * 8)
+    wd, ud, dd, ob = own.weight(w.tensor()), own.weight(w2.tensor()), own.weight(w.tensor(dense=True)), own.u32([0, T])
+    with gpu.batch() as b:
+        b.expert_swiglu_q8(wd, ud, x, ob, None, 1, q)
+        b.matmul_q8(dd, x, y)
+        b.matmul_q8(dd, x, z, BF16)
+    qc, qs = gpu.read_rows8(q)
+    got, half = gpu.read(y).reshape(T, 16), read_bf16(gpu, z).reshape(T, 16)
+    for r, c, s in ((slice(T - last, T), tail, tb), (slice(0, 512), few, fb), (slice(T - 1024, T - 512), few, fb)):
+        v = rows_value(c, s)
+        check_quantized(qc[r], qs[r], *swiglu64(v, w, w2, 0))
+        check_rows(got[r], *product(v, w.value()), n_in, False)
+        check_rows(half[r], *product(v, w.value()), n_in, True)
+
+
+def test_norm_q8_of_more_rows_than_a_launch_is_wide(gpu, own):
+    rng = np.random.default_rng(13)
+    rows, n = (1 << 24) + 5, 16
+    x, q = own.zeros(rows * n), own.rows8(rows, n)
+    norm = own.weight(Tensor.dense([n], np.ones(n, np.float32)))
+    at = [0, (1 << 22) - 1, 1 << 22, (1 << 24) - 1, rows - 1]
+    v = rng.standard_normal((len(at), n)).astype(np.float32)
+    for r, i in zip(v, at):
+        gpu.write(x.view(i * n, n), r)
+    with gpu.batch() as b:
+        b.norm_q8(x, None, norm, None, None, q, 1e-6)
+    c, s = gpu.read_rows8(q)
+    want = norm64(v, np.ones(n), 1e-6)
+    check_quantized(c[at], s[at], want, 70 * U * np.abs(want))
+    rest = np.ones(rows, bool)
+    rest[at] = False
+    assert not c[rest].any() and np.all(s[rest] == 0x0080)   # the least scale, 2^-126
+
+
 # -------------------------------------------------------------------- mix --
 @pytest.mark.parametrize("T,K,h", [(1, 1, 16), (1, 10, 2048), (3, 8, 130), (5, 3, 7), (64, 10, 512), (300, 2, 1028)])
 @pytest.mark.parametrize("x_type", [F32, BF16])
@@ -532,7 +751,8 @@ def chain_state(own, rng, T, h, E, K, ff, ytype):
 
 
 @pytest.mark.parametrize("T,h,E,K,ff,ytype", [(1, 256, 8, 2, 128, F32), (7, 272, 5, 3, 48, F32),
-                                              (70, 256, 6, 4, 144, BF16), (200, 128, 4, 2, 256, BF16)])
+                                              (70, 256, 6, 4, 144, BF16), (200, 128, 4, 2, 256, BF16),
+                                              (700, 256, 6, 4, 144, BF16), (1300, 128, 5, 4, 128, F32)])
 def test_chain(gpu, own, T, h, E, K, ff, ytype):
     """The operators as a block uses them, each stage against 64 bits over what
     the stage before it wrote; then captured and replayed over new inputs."""
