@@ -35,9 +35,7 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 
-constexpr int kThreads = 256;  // of the quantising launch
-
-enum { SWIGLU = 0, F32OUT = 1, BF16OUT = 2, ACT = 3 };  // ACT: SwiGLU as F32 rows
+enum { SWIGLU = 0, F32OUT = 1, BF16OUT = 2, ACT = 3 };  // ACT: SWIGLU whose blocks hold less than the 128 outputs of a scale
 
 struct Args {
     const uint8_t *w, *w2;        // codes (w2: the up weights of SWIGLU)
@@ -46,11 +44,13 @@ struct Args {
     const uint16_t *xs;           // and scales [xrows, kb]
     const uint32_t *offsets;      // [experts + 1], or null: one segment of all positions
     const uint32_t *perm;         // [P] pair of each position, or null: the position itself
-    void *y;                      // F32OUT / BF16OUT: [P, out]
+    void *y;                      // F32OUT / BF16OUT: [P, out]; ACT: F32 rows on the way
+    uint32_t *arrived;            // ACT: counts, zero between launches
     uint8_t *codes;               // SWIGLU: [P, out] and scales [P, ceil(out / 128)]
     uint16_t *scales;
     uint32_t stype, xrows, in, out, kb, experts, P, kdiv;
     uint32_t col_tiles;           // tiles along the outputs
+    uint32_t tiles;               // at most this many along the positions
 };
 
 // The work of a block: items, each an M-tile (a run of at most BM positions of a
@@ -69,7 +69,8 @@ struct Tile {
 };
 constexpr uint32_t kXcds = 8, kPanel = 4;
 template <int BM, int NW>
-__device__ __forceinline__ uint32_t find_items(const Args &a, uint32_t from, uint32_t kMax, Tile *out, uint32_t *lds /* NW */) {
+__device__ __forceinline__ uint32_t find_items(const Args &a, uint32_t from, uint32_t kMax, Tile *out, uint32_t *lds /* NW */,
+                                               uint32_t *number = nullptr) {
     const uint32_t tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     const uint32_t per = (a.experts + 64 * NW - 1) / (64 * NW), e0 = tid * per;
     auto seg = [&](uint32_t e, uint32_t &lo, uint32_t &n) {
@@ -101,7 +102,9 @@ __device__ __forceinline__ uint32_t find_items(const Args &a, uint32_t from, uin
             total += lds[v];
         }
     }
-    // (fewer than 2^31 items: the launch checks it)
+    // (fewer than 2^31 items: the launch checks it.  Segments that overlap can make
+    // more tiles than the launch has blocks for: the last are left out, whole.)
+    total = min(total, a.tiles);
     const uint32_t items = total * a.col_tiles, range = (items + kXcds - 1) / kXcds;
     const uint32_t lo_item = blockIdx.x % kXcds * range, hi_item = min(items, lo_item + range);
     const uint32_t turn = gridDim.x / kXcds;
@@ -109,15 +112,16 @@ __device__ __forceinline__ uint32_t find_items(const Args &a, uint32_t from, uin
     if (first >= hi_item) return 0;
     const uint32_t n = min(kMax, (hi_item - first + turn - 1) / turn);
     // item `i` of a segment of k tiles
-    auto put = [&](uint32_t s, uint32_t e, uint32_t lo, uint32_t hi, uint32_t k, uint32_t i) {
+    auto put = [&](uint32_t s, uint32_t e, uint32_t lo, uint32_t hi, uint32_t k, uint32_t first_tile, uint32_t i) {
         const uint32_t panel = k < 2 * kPanel || a.col_tiles <= 2 * kPanel ? a.col_tiles : kPanel;
         const uint32_t ct = i / (k * panel) * panel;
         const uint32_t wide = min(panel, a.col_tiles - ct), at = i - k * ct;
         const uint32_t m0 = lo + at / wide * BM;
+        if (number) *number = first_tile + at / wide;
         out[s] = Tile{e, m0, hi - m0 < BM ? hi : m0 + BM, ct + at % wide};
     };
     if (!a.offsets) {
-        if (tid < n) put(tid, 0, 0, a.P, total, first + tid * turn);
+        if (tid < n) put(tid, 0, 0, a.P, total, 0, first + tid * turn);
     } else {
         for (uint32_t s = 0; s < n; s++) {
             const uint32_t item = first + s * turn, tile = item / a.col_tiles;
@@ -127,7 +131,7 @@ __device__ __forceinline__ uint32_t find_items(const Args &a, uint32_t from, uin
                 uint32_t lo, k;
                 const uint32_t hi = seg(e0 + i, lo, k);
                 if (tile - at < k) {
-                    put(s, e0 + i, lo, hi, k, item - at * a.col_tiles);
+                    put(s, e0 + i, lo, hi, k, at, item - at * a.col_tiles);
                     break;
                 }
                 at += k;
@@ -138,12 +142,13 @@ __device__ __forceinline__ uint32_t find_items(const Args &a, uint32_t from, uin
     return n;
 }
 // The one item of a block in a grid with a block per item.
-constexpr int kFind = 12;  // its words of LDS
+constexpr int kFind = 13;  // its words of LDS
 template <int BM, int NW>
-__device__ __forceinline__ bool find_tile(const Args &a, Tile &t, uint32_t *lds) {
-    static_assert(NW + 4 <= kFind, "LDS words");
+__device__ __forceinline__ bool find_tile(const Args &a, Tile &t, uint32_t &number, uint32_t *lds) {
+    static_assert(NW + 5 <= kFind, "LDS words");
     Tile *out = reinterpret_cast<Tile *>(lds + NW);
-    if (find_items<BM, NW>(a, 0, 1, out, lds) == 0) return false;
+    if (find_items<BM, NW>(a, 0, 1, out, lds, lds + NW + 4) == 0) return false;
+    number = __builtin_amdgcn_readfirstlane(lds[NW + 4]);
     t.e = __builtin_amdgcn_readfirstlane(out->e);
     t.m0 = __builtin_amdgcn_readfirstlane(out->m0);
     t.end = __builtin_amdgcn_readfirstlane(out->end);
@@ -302,6 +307,17 @@ __device__ __forceinline__ void store_swiglu(const Args &a, const f32x4q (&acc)[
     }
 }
 
+// Two values, 8-byte aligned, to and from what every XCD sees.
+__device__ __forceinline__ void store_agent(float *p, float a, float b) {
+    const uint64_t v = (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
+    __hip_atomic_store(reinterpret_cast<uint64_t *>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void load_agent(const float *p, float &a, float &b) {
+    const uint64_t v =
+        __hip_atomic_load(reinterpret_cast<const uint64_t *>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    a = __uint_as_float((uint32_t)v), b = __uint_as_float((uint32_t)(v >> 32));
+}
+
 // Few rows per expert: the time is the weights' way from memory, so what counts
 // is how many of their loads are in flight.  A wave owns RT row tiles (SWIGLU: 16
 // gate rows and their up rows) and a range of the blocks of 128 columns (KS waves
@@ -339,7 +355,8 @@ __global__ __launch_bounds__(64 * NW, WPS) void stream_kernel(Args a) {
     static_assert(RG * kCols <= 128 && 128 % (RG * kCols) == 0, "a block's rows share their scales");
     __shared__ __attribute__((aligned(16))) StreamLds<MODE, RT, TT, KS, NW> lds;
     Tile t;
-    if (!find_tile<BM, NW>(a, t, lds.find)) return;
+    uint32_t number;
+    if (!find_tile<BM, NW>(a, t, number, lds.find)) return;
     const uint32_t tid = threadIdx.x, lane = tid & 63, c = lane & 15, q = lane >> 4;
     const uint32_t wv = __builtin_amdgcn_readfirstlane(tid >> 6), rg = wv / KS, ks = wv % KS;
     const uint32_t n0 = t.ct * (RG * kCols) + rg * kCols, nb = min(n0, a.out - 1);
@@ -455,26 +472,67 @@ __global__ __launch_bounds__(64 * NW, WPS) void stream_kernel(Args a) {
                     *reinterpret_cast<f32x4q *>(r + ((j * TT + i) * 64 + lane) * 4) = acc[j][i];
         }
         __syncthreads();
-        if (ks > 0) return;
+        if (MODE != ACT && ks > 0) return;
 #pragma unroll
         for (int v = 0; v < KS - 1; v++)
 #pragma unroll
             for (int j = 0; j < RT; j++)
 #pragma unroll
                 for (int i = 0; i < TT; i++)
-                    acc[j][i] += *reinterpret_cast<const f32x4q *>(lds.red[rg * (KS - 1) + v] + ((j * TT + i) * 64 + lane) * 4);
+                    if (ks == 0) acc[j][i] += *reinterpret_cast<const f32x4q *>(lds.red[rg * (KS - 1) + v] + ((j * TT + i) * 64 + lane) * 4);
     }
     if constexpr (MODE == SWIGLU)
         store_swiglu<RT, TT, NW>(a, acc, to, n0 + 4 * q, t.ct, wv, lds.tops);
     else if constexpr (MODE == ACT) {
-        if (n0 + 4 * q >= a.out) return;  // (out is a multiple of 16)
+        // The block's outputs as F32 rows; the last block of the 128 that share a
+        // scale quantises them.  The rows are stored and loaded past the caches of
+        // one XCD (agent scope) and the stores have landed (vmcnt) before the count:
+        // fences, which write back and drop a whole L2, took 30 us here.
+        float *const rows = static_cast<float *>(a.y);
 #pragma unroll
         for (int i = 0; i < TT; i++) {
-            if (to[i] == 0xffffffffu) continue;
+            if (ks > 0 || to[i] == 0xffffffffu || n0 + 4 * q >= a.out) continue;  // (out is a multiple of 16)
             f32x4q v;
 #pragma unroll
             for (int e = 0; e < 4; e++) v[e] = swiglu_of(acc[0][i][e], acc[1][i][e]);
-            *reinterpret_cast<f32x4q *>(static_cast<float *>(a.y) + (uint64_t)to[i] * a.out + n0 + 4 * q) = v;
+            float *const at = rows + (uint64_t)to[i] * a.out + n0 + 4 * q;
+            store_agent(at, v[0], v[1]);
+            store_agent(at + 2, v[2], v[3]);
+        }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        constexpr uint32_t kOuts = RG * kCols;  // outputs of a block
+        const uint32_t group = t.ct * kOuts / 128, cols = min(128u, a.out - 128 * group);
+        if (tid == 0) {
+            uint32_t *const count = a.arrived + number * ob + group;
+            const bool last = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+                              (cols + kOuts - 1) / kOuts - 1;
+            if (last) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            lds.find[0] = last;
+        }
+        __syncthreads();
+        if (!lds.find[0]) return;
+        // 16 lanes hold the columns of a row, eight each
+#pragma unroll
+        for (int r = 0; r < BM; r += 4 * NW) {
+            const uint32_t p = t.m0 + r + tid / 16, col = tid % 16 * 8;
+            const bool row = p < t.end && (a.perm ? a.perm[p] : p) / a.kdiv < a.xrows, live = row && col < cols;
+            const float *const from = rows + (uint64_t)p * a.out + 128 * group + col;
+            float v[8] = {};
+            if (live) {
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) load_agent(from + j, v[j], v[j + 1]);
+            }
+            uint32_t top = 0;
+#pragma unroll
+            for (int j = 0; j < 8; j++) top = max(top, abs_word(v[j]));
+            const uint32_t sb = q8_scale_bits(row16_max(top));
+            if (!live) continue;
+            const float inv = q8_inverse(sb);
+            *reinterpret_cast<u32x2q *>(a.codes + (uint64_t)p * a.out + 128 * group + col) =
+                u32x2q{q8_codes4(v[0], v[1], v[2], v[3], inv), q8_codes4(v[4], v[5], v[6], v[7], inv)};
+            if (col == 0) a.scales[(uint64_t)p * ob + group] = (uint16_t)sb;
         }
     } else
         store_rows<MODE, RT, TT>(a, acc, to, n0 + 4 * RT * q);
@@ -868,41 +926,6 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
     }
 }
 
-// F32 rows of the positions that a segment holds, in 8 bits; one block per
-// position.  16 lanes hold the 128 columns of a scale.
-__global__ __launch_bounds__(kThreads) void quantize_kernel(Args a, const float *act) {
-    __shared__ uint32_t held;
-    const uint32_t p = blockIdx.x, tid = threadIdx.x;
-    if (tid == 0) held = 0;
-    __syncthreads();
-    uint32_t mine = 0;
-    for (uint32_t e = tid; e < a.experts; e += kThreads) mine |= a.offsets[e] <= p && p < a.offsets[e + 1];
-    if (mine) held = 1;
-    const uint32_t pair = a.perm ? a.perm[p] : p, ob = (a.out + 127) / 128;
-    const bool row = pair / a.kdiv < a.xrows;
-    __syncthreads();
-    if (!held || !row) return;
-    for (uint32_t i = 8 * tid; (i & ~127u) < a.out; i += 8 * kThreads) {
-        float v[8] = {};
-        const bool live = i < a.out;  // (out is a multiple of 16)
-        const float *from = act + (uint64_t)p * a.out + i;
-        if (live) {
-            const f32x4q lo = *reinterpret_cast<const f32x4q *>(from), hi = *reinterpret_cast<const f32x4q *>(from + 4);
-#pragma unroll
-            for (int j = 0; j < 4; j++) v[j] = lo[j], v[4 + j] = hi[j];
-        }
-        uint32_t top = 0;
-#pragma unroll
-        for (int j = 0; j < 8; j++) top = max(top, abs_word(v[j]));
-        const uint32_t sb = q8_scale_bits(row16_max(top));
-        if (!live) continue;
-        const float r = q8_inverse(sb);
-        *reinterpret_cast<u32x2q *>(a.codes + (uint64_t)p * a.out + i) =
-            u32x2q{q8_codes4(v[0], v[1], v[2], v[3], r), q8_codes4(v[4], v[5], v[6], v[7], r)};
-        if ((tid & 15) == 0) a.scales[(uint64_t)p * ob + i / 128] = (uint16_t)sb;
-    }
-}
-
 }  // namespace q8
 
 // The stream kernel's forms of one mode: its outputs per block and its kernel.
@@ -937,6 +960,7 @@ static Form stream_form(uint32_t out, uint32_t kb, uint64_t tiles) {
 static hipError_t launch_form(Prof *p, hipStream_t s, const char *name, const Form &f, uint64_t tiles, q8::Args a,
                               uint64_t most_blocks = 0x7ffffff8) {
     a.col_tiles = (a.out + f.cols - 1) / f.cols;
+    a.tiles = (uint32_t)tiles;
     uint64_t blocks = (tiles * a.col_tiles + q8::kXcds - 1) / q8::kXcds * q8::kXcds;
     if (blocks > 0x7ffffff8ull) return hipErrorInvalidConfiguration;
     if (blocks > most_blocks) blocks = most_blocks;
@@ -944,10 +968,8 @@ static hipError_t launch_form(Prof *p, hipStream_t s, const char *name, const Fo
     return launch_kernel(p, name, f.kernel, dim3((uint32_t)blocks), dim3(f.threads), 0, s, a);
 }
 
-// scratch: F32 values for the two-launch SwiGLU of few positions
 template <int MODE>
-static hipError_t launch_q8(Prof *p, hipStream_t s, const char *name, q8::Args a, float *scratch = nullptr,
-                            uint64_t scratch_len = 0) {
+static hipError_t launch_q8(Prof *p, hipStream_t s, const char *name, q8::Args a) {
     using namespace q8;
     a.kb = (a.in + 127) / 128;
     const uint32_t experts = a.offsets ? a.experts : 1;
@@ -956,17 +978,19 @@ static hipError_t launch_q8(Prof *p, hipStream_t s, const char *name, q8::Args a
     auto max_tiles = [&](uint32_t bm) { return a.P / bm + (a.offsets ? live : (uint64_t)(a.P % bm != 0)); };
     // Tiles of 128 rows need CUs to work on them: enough items, or enough rows
     // (2048 columns, microseconds of tiles against the best stream form):
-    //   SwiGLU  512 outputs, 1 expert, 512 rows (16 items): 19.0, 16.1;  4 experts, 1024 rows (32): 19.5, 26.2
-    //           768 outputs, 16 experts, 64 rows (96 items): 15.7, 17.8;  2048 rows: 21.7, 73.6
+    //   SwiGLU  512 outputs, 1 expert, 512 rows (16 items): 19.1, 15.4;  4 experts, 1024 rows (32): 19.9, 46.3
+    //           768 outputs, 16 experts, 16 rows (96 items): 15.2, 11.2;  128 rows: 15.6, 16.6;  256 rows: 15.5, 20.5
+    //           512 outputs, 512 experts, 20 rows (80 items): 15.5, 14.6;  40 rows (160): 18.7, 22.9
     //   bf16    4096 outputs, 128 rows (16 items): 16.8, 13.6;  256 rows (32): 17.3, 24.3
     //           16384 outputs, 32 rows (64 items): 14.2, 13.8;  48 rows: 14.2, 24.4
     //   F32     4096 outputs, 256 rows (32 items): 31.6, 25.4;  512 rows (64): 34.0, 38.3
     // and an expert's rows to be worth its steps (768 columns to 2048, 64 experts):
     //   bf16    512 rows: 21.6, 18.9;  1024: 21.9, 24.9      F32  512 rows: 24.4, 19.9;  1024: 24.8, 26.1
-    // SwiGLU's steps are worth it from the first row on (2048 to 512, 512 experts: 40 rows 17.5, 21.8;
-    // 640: 131, 131).  DMA offsets are 32-bit.
+    // SwiGLU's steps are worth it from the first row on (2048 to 512, 512 experts: 640 rows 132, 144).
+    // DMA offsets are 32-bit.
     constexpr uint64_t kRows = MODE == SWIGLU ? 0 : MODE == F32OUT ? 16 : 12;
-    const bool fills = ct * a.P >= (MODE == F32OUT ? 5120 : 2560) || (MODE != F32OUT && ct * live >= 80);
+    const bool fills = ct * a.P >= (MODE == F32OUT ? 5120 : 2560) || (MODE == BF16OUT && ct * live >= 80) ||
+                       (MODE == SWIGLU && ct * (a.P + 32 * live) >= 3520);
     const bool tiled = fills && a.P >= kRows * experts && (uint64_t)a.xrows * a.in < 0xffffffffull &&
                        (uint64_t)a.out * a.in < 0xffffffffull;
     // Two token tiles a wave read the weights half as often, where that leaves 256
@@ -978,17 +1002,11 @@ static hipError_t launch_q8(Prof *p, hipStream_t s, const char *name, q8::Args a
     const uint64_t tiles = max_tiles(two ? 32 : 16);
     if constexpr (MODE == SWIGLU) {
         // A scale needs 128 outputs: blocks that hold them (512 KiB of weights at
-        // 2048 columns) are few, so blocks of 16 to 64 write F32 rows and a second
-        // launch quantises them.  (What does not fit has 2^32 bytes of rows or weights.)
-        if ((uint64_t)a.P * a.out <= scratch_len) {
-            Args b = a;
-            b.y = scratch;
-            const hipError_t e = launch_form(p, s, name, two ? stream_form<ACT, 2>(a.out, a.kb, tiles)
-                                                             : stream_form<ACT, 1>(a.out, a.kb, tiles), tiles, b);
-            if (e != hipSuccess) return e;
-            return launch_kernel(p, "quantize_q8", quantize_kernel, dim3(a.P), dim3(kThreads), 0, s, a,
-                                 (const float *)scratch);
-        }
+        // 2048 columns) are few, so blocks of 16 to 64 write F32 rows and the last
+        // of each 128 quantises them.  (What does not fit has 2^32 bytes of rows or weights.)
+        if ((uint64_t)a.P * a.out <= kQ8RowsLen && tiles * ((a.out + 127) / 128) <= kQ8CountLen)
+            return launch_form(p, s, name, two ? stream_form<ACT, 2>(a.out, a.kb, tiles) : stream_form<ACT, 1>(a.out, a.kb, tiles),
+                               tiles, a);
         return launch_form(p, s, name, stream_form<SWIGLU, 1>(a.out, a.kb, max_tiles(16)), max_tiles(16), a);
     } else {
         return launch_form(p, s, name, two ? stream_form<MODE, 2>(a.out, a.kb, tiles) : stream_form<MODE, 1>(a.out, a.kb, tiles),
@@ -1007,14 +1025,15 @@ hipError_t launch_q8_rows(Prof *p, hipStream_t s, const char *name, const Q8Weig
 
 hipError_t launch_q8_swiglu(Prof *p, hipStream_t s, const Q8Weight &gate, const Q8Weight &up, const Q8Rows &x,
                             const uint32_t *offsets, const uint32_t *perm, uint32_t k, const Q8Rows &out,
-                            float *scratch, uint64_t scratch_len) {
+                            float *rows, uint32_t *arrived) {
     q8::Args a{};
     a.w = gate.codes, a.ws = gate.scales, a.w2 = up.codes, a.ws2 = up.scales, a.stype = gate.stype;
     a.in = gate.in, a.out = gate.out, a.experts = gate.experts;
     a.x = x.codes, a.xs = x.scales, a.xrows = x.rows, a.P = out.rows;
     a.offsets = offsets, a.perm = perm, a.kdiv = k;
     a.codes = out.codes, a.scales = out.scales;
-    return launch_q8<q8::SWIGLU>(p, s, "expert_swiglu_q8", a, scratch, scratch_len);
+    a.y = rows, a.arrived = arrived;
+    return launch_q8<q8::SWIGLU>(p, s, "expert_swiglu_q8", a);
 }
 
 }  // namespace moehip

@@ -283,10 +283,12 @@ hipError_t launch_mix_tokens(Prof *p, hipStream_t s, const void *x, bool bf16, c
 hipError_t launch_q8_rows(Prof *p, hipStream_t s, const char *name, const Q8Weight &w, const Q8Rows &x,
                           const uint32_t *offsets, const uint32_t *perm, void *y, bool bf16);
 // out[p] = silu(x_t . G_e) * (x_t . U_e), t = perm[p] / k (perm null: p);
-// scratch: room for F32 rows of few positions
+// rows, arrived: an engine's kQ8RowsLen floats and kQ8CountLen counts, zero between
+// launches, for few positions
+constexpr uint64_t kQ8RowsLen = 2560 * 128, kQ8CountLen = 22528;
 hipError_t launch_q8_swiglu(Prof *p, hipStream_t s, const Q8Weight &gate, const Q8Weight &up, const Q8Rows &x,
                             const uint32_t *offsets, const uint32_t *perm, uint32_t k, const Q8Rows &out,
-                            float *scratch, uint64_t scratch_len);
+                            float *rows, uint32_t *arrived);
 
 // ---- fused single-token decode (k_decode.hip) ----
 struct DecodeArgs {

@@ -516,9 +516,40 @@ def test_shared_expert_and_rows_named_twice(gpu, own, T):
         assert np.isnan(got2[row]).all() if at.size == 0 else (got2[row] == got[at]).any(0).all()
 
 
+@pytest.mark.parametrize("T,n_in,ff,E", [(1, 512, 512, 1), (10, 2048, 512, 10), (48, 512, 272, 4), (300, 256, 144, 2)])
+def test_small_swiglu_over_and_over(gpu, own, T, n_in, ff, E):
+    """The blocks that share a scale hand their rows to the last of them: the
+    same bits in each of many calls in flight, by call and from a replayed graph,
+    also after segments that overlap (more tiles than the launch has blocks for)."""
+    rng = np.random.default_rng(T + ff)
+    w, w2 = Weight8(rng, E, ff, n_in), Weight8(rng, E, ff, n_in)
+    codes, bits = random_rows(rng, T, n_in)
+    offsets = np.sort(np.r_[0, rng.integers(0, T + 1, E - 1), T])
+    wd, ud, x, ob = own.weight(w.tensor()), own.weight(w2.tensor()), own.rows8(T, n_in, codes, bits), own.u32(offsets)
+    over = own.u32(np.arange(E + 1) % 2 * T)
+    many = [own.rows8(T, ff) for _ in range(24)]
+    cap = gpu.capture()
+    with cap as b:
+        for q in many[:8]:
+            b.expert_swiglu_q8(wd, ud, x, ob, None, 1, q)
+    want, dw = (np.concatenate(v) for v in zip(*(swiglu64(rows_value(codes, bits)[a:c], w, w2, e)
+                                                for e, (a, c) in enumerate(zip(offsets[:-1], offsets[1:])))))
+    for turn in range(4):
+        with gpu.batch() as b:
+            b.expert_swiglu_q8(wd, ud, x, over, None, 1, many[23])
+            b.graph(cap.graph)
+            for q in many[8:]:
+                b.expert_swiglu_q8(wd, ud, x, ob, None, 1, q)
+        got = [gpu.read_rows8(q) for q in many]
+        check_quantized(*got[0], want, dw)
+        for c, s in got[1:]:
+            assert np.array_equal(c, got[0][0]) and np.array_equal(s, got[0][1])
+    cap.graph.destroy()
+
+
 def test_two_gpus_at_once(gpu, own):
     """Batches of two engines on one device, both in flight: neither sees the
-    other's rows between the two launches of a small SwiGLU."""
+    other's rows on their way to 8 bits in a small SwiGLU."""
     rng = np.random.default_rng(17)
     T, n_in, ff, E = 48, 512, 512, 4
     w, w2 = Weight8(rng, E, ff, n_in), Weight8(rng, E, ff, n_in)
