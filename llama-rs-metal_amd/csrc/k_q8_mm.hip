@@ -562,13 +562,14 @@ __global__ __launch_bounds__(64 * NW, WPS) void stream_kernel(Args a) {
 // 42.6 to 52.9 where all at once took 40.4; wave priorities: no difference.)
 typedef __attribute__((address_space(3))) void *lds_ptr;
 constexpr uint64_t kCus = 256;
-constexpr int kGroup = 8, kStages = 3, kTileWaves = 8, kTileRows = 128, kTileCols = 256, kSlots = 8;
+constexpr uint32_t kStage = 128 * 128;  // bytes of a stage's token rows, half of its weight rows'
+constexpr int kScaleSlots = 32, kGroup = 8, kStages = 3, kTileWaves = 8, kTileRows = 128, kTileCols = 256, kSlots = 8;
 
 struct TileLds {
-    uint8_t x[kStages][kTileRows * 128];
-    uint8_t w[kStages][kTileCols * 128];
-    uint16_t sx[4][kGroup][kTileRows];  // scales of kGroup steps: of the four steps from the current one on
-    float sw[4][2][kGroup];
+    uint8_t x[kStages * kStage];
+    uint8_t w[2 * kStages * kStage];
+    uint16_t sx[kScaleSlots][kTileRows];  // scales by step, in a ring of four groups of kGroup steps
+    float sw[kScaleSlots][2];
     uint32_t tops[4 * kTileRows];
     uint32_t map[kSlots][kTileRows];  // SWIGLU: input row of each position; else its output row; 0xffffffff: none
     Tile slot[kSlots];
@@ -618,15 +619,16 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
     // columns past `in` in the last step: a chunk is replaced by its row's first of
     // the block, and the weights' codes are zeroed when they are used
     const uint32_t back = TAIL && dchunk >= tail ? dchunk : 0;
-    // one of the kLoads instructions of block kb into `stage`
-    auto load = [&](int i, uint32_t stage, uint32_t kb) {
-        const uint32_t b = TAIL && kb + 1 == nk ? back : 0;
+    // one of the kLoads instructions of the block at column k into the stage at `to`
+    // (stages are named by where their token rows start)
+    auto load = [&](int i, uint32_t to, uint32_t k) {
+        const uint32_t b = TAIL && k + 128 > a.in ? back : 0;
         if (i < NX)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lds_ptr)(lds.x[stage] + (64 * i + 8 * wv) * 128), 16,
-                                                     xoff[i < NX ? i : 0] - b, kb * 128, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lds_ptr)(lds.x + to + (64 * i + 8 * wv) * 128), 16,
+                                                     xoff[i < NX ? i : 0] - b, k, 0, 0);
         else
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_ptr)(lds.w[stage] + (64 * (i - NX) + 8 * wv) * 128), 16,
-                                                     woff[i < NX ? 0 : i - NX] - b, kb * 128, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_ptr)(lds.w + 2 * to + (64 * (i - NX) + 8 * wv) * 128), 16,
+                                                     woff[i < NX ? 0 : i - NX] - b, k, 0, 0);
     };
     // the thread's share of the scales of kGroup steps: kSr neighbouring steps of one row
     constexpr int kSr = kTileRows * kGroup / (64 * kTileWaves);
@@ -646,39 +648,38 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
     };
     auto keep_scales = [&](uint32_t buf) {
 #pragma unroll
-        for (int i = 0; i < kSr; i++) lds.sx[buf][sk + i][srow] = sr[i];
-        if (has_sw) lds.sw[buf][tid / kGroup][tid % kGroup] = swr;
+        for (int i = 0; i < kSr; i++) lds.sx[buf + sk + i][srow] = sr[i];
+        if (has_sw) lds.sw[buf + tid % kGroup][tid / kGroup] = swr;
     };
     // a lane's chunks of its row in tile 0 of a wave's rows
     const uint32_t lo = c * 128 + ((q ^ (c >> 1)) << 4), hi = c * 128 + (((q + 4) ^ (c >> 1)) << 4);
-    const uint8_t *const xbase = lds.x[0] + 16 * tg * 128, *const wbase = lds.w[0] + 64 * wg * 128;
+    const uint8_t *const xbase = lds.x + 16 * tg * 128, *const wbase = lds.w + 64 * wg * 128;
     auto codes = [&](const uint8_t *rows) {
         return Codes{*reinterpret_cast<const u32x4q *>(rows + lo), *reinterpret_cast<const u32x4q *>(rows + hi)};
     };
-    auto weights = [&](uint32_t stage, int j) { return codes(wbase + stage * (kTileCols * 128) + j * 2048); };
-    auto tokens = [&](uint32_t stage, int i) { return codes(xbase + stage * (kTileRows * 128) + i * 4096); };
+    auto weights = [&](uint32_t stage, int j) { return codes(wbase + 2 * stage + j * 2048); };
+    auto tokens = [&](uint32_t stage, int i) { return codes(xbase + stage + i * 4096); };
     // What a wave holds of a step: its scales, raw, and its codes of NS token tiles
     // (tile i: rows 32 i + 16 tg on) and four row tiles.
     struct Scales {
         float sw, sw2;
         uint32_t sx[4];
     };
-    auto scales = [&](auto &sc, uint32_t kb, uint32_t grp) {
-        sc.sw = lds.sw[grp][MODE == SWIGLU ? 0 : wg >> 1][kb % kGroup];
-        sc.sw2 = MODE == SWIGLU ? lds.sw[grp][1][kb % kGroup] : 0.f;
+    auto scales = [&](auto &sc, uint32_t slot) {
+        sc.sw = lds.sw[slot][MODE == SWIGLU ? 0 : wg >> 1];
+        sc.sw2 = MODE == SWIGLU ? lds.sw[slot][1] : 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; i++) sc.sx[i] = lds.sx[grp][kb % kGroup][32 * i + 16 * tg + c];
+        for (int i = 0; i < 4; i++) sc.sx[i] = lds.sx[slot][32 * i + 16 * tg + c];
     };
     // A step over codes wc, xc and scales sc; each is replaced by the next step's
-    // after its last use (from stage `next` and the scales' buffer ngrp), and
-    // `between`, after the first products, turns to the step to load,
-    // whose DMA is issued from there on (in one go it held the waves up until
-    // the memory pipe had taken all of it; none without `loads`).  A block's sums join their running
+    // after its last use (from stage `next` and the scales' slot), and issue(i),
+    // i <= kLoads, is called along the products (a step's DMA in one go held the waves
+    // up until the memory pipe had taken all of it).  A block's sums join their running
     // sums kLag products later.  In this order the matrix cores wait for neither.
-    auto compute = [&](auto &acc, Codes (&wc)[4], auto &xc, Scales &sc, uint32_t next, uint32_t kb, uint32_t ngrp,
-                       bool loads, auto between) {
+    auto compute = [&](auto &acc, Codes (&wc)[4], auto &xc, Scales &sc, uint32_t next, uint32_t slot, bool last,
+                       auto issue) {
         constexpr int NS = sizeof(acc[0]) / sizeof(acc[0][0]), kLag = 3;
-        if (TAIL && kb + 1 == nk) {
+        if (TAIL && last) {
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 if (16 * q >= tail) wc[j].lo = u32x4q{0, 0, 0, 0};
@@ -693,7 +694,6 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
             s2[i] = MODE == SWIGLU ? bf16_to_f32(sc.sx[i]) * sc.sw2 : 0.f;
         }
         f32x4q d[4 * NS];
-        uint32_t lstage = 0, lkb = 0;
 #pragma unroll
         for (int n = 0; n < 4 * NS + kLag; n++) {
             const int i = n / 4, j = n % 4;
@@ -701,13 +701,12 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
                 d[n] = block_dot(wo[j], Operand<kF16>(xc[i]));
                 if (i == NS - 1) wc[j] = weights(next, j);
                 if (j == 3) xc[i] = tokens(next, i);
-                if (n == 1 && loads) between(lstage, lkb);
-                if (n == 3) scales(sc, kb + 1, ngrp);
+                if (n == 1) issue(0);
+                if (n == 3) scales(sc, slot);
                 if (n >= 3) {
                     constexpr int R = 4 * NS - 3;
 #pragma unroll
-                    for (int l = (n - 3) * kLoads / R; l < (n - 2) * kLoads / R; l++)
-                        if (loads) load(l, lstage, lkb);
+                    for (int l = (n - 3) * kLoads / R; l < (n - 2) * kLoads / R; l++) issue(l + 1);
                 }
             }
             if (n >= kLag) {
@@ -735,29 +734,32 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
         }
         __syncthreads();
         // the step that is loaded next: slot ps (past the last: the last again,
-        // unused), block pk; the stage it goes to; its scales' buffer
-        uint32_t ps = 0, pk = 0, pstage = 0, pgrp = 3, grp = 3, stage = 0;
-        bool pending = false;
-        // aims at the step that is loaded next; its scales are loaded before it, so
-        // that the wait for it covers them
-        auto aim_next = [&] {
-            if (pk % kGroup == 0) {
-                if (pk == 0) aim(min(ps, slots - 1));
-                load_scales(min(ps, slots - 1), pk);
-                pending = true;
-                pgrp = (pgrp + 1) % 4;
+        // unused), column pk; whether it begins a group of scales; the group's ring slot
+        uint32_t ps = 0, pk = 0, pslot = kScaleSlots - kGroup;
+        bool due = true, pending = false;
+        const uint32_t columns = nk * 128;
+        // part i of its loads, in order 0 .. kLoads: its scales come first, so that the
+        // wait for it covers them
+        auto load_part = [&](int i, uint32_t to) {
+            if (i == 0) {
+                if (due) {
+                    if (pk == 0) aim(min(ps, slots - 1));
+                    load_scales(min(ps, slots - 1), pk / 128);
+                    pslot = (pslot + kGroup) % kScaleSlots;
+                }
+                pending = due;
+                __builtin_amdgcn_sched_barrier(0);
+            } else {
+                load(i - 1, to, pk);
             }
-            __builtin_amdgcn_sched_barrier(0);
+            if (i < kLoads) return;
+            pk += 128;
+            if (pk == columns) pk = 0, ps++;
+            due = pk % (kGroup * 128) == 0;
         };
-        auto loaded = [&] {
-            pstage = pstage == kStages - 1 ? 0 : pstage + 1;
-            if (++pk == nk) pk = 0, ps++;
-        };
-        auto ahead = [&] {
-            aim_next();
+        auto ahead = [&](uint32_t to) {
 #pragma unroll
-            for (int i = 0; i < kLoads; i++) load(i, pstage, pk);
-            loaded();
+            for (int i = 0; i <= kLoads; i++) load_part(i, to);
         };
         auto barrier = [&] {  // of LDS traffic only: the loads stay in flight
             __builtin_amdgcn_sched_barrier(0);
@@ -768,8 +770,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
             __builtin_amdgcn_sched_barrier(0);
         };
         auto store_scales = [&] {
-            if (pending) keep_scales(pgrp);
-            pending = false;
+            if (pending) keep_scales(pslot);
         };
         // A step begins when the next one's rows are in LDS and this one's are read
         // out: all but the loads of the step after the next have landed (gfx9
@@ -783,12 +784,15 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
             store_scales();
             barrier();
         };
-        ahead();
+        ahead(0);
         store_scales();
-        ahead();
+        ahead(kStage);
         begin();
-        ahead();
-        // An item's outputs, through LDS buffer `buf`: a lane's results are neighbours
+        ahead(2 * kStage);
+        // the stages of the step at work and of the next one; the ring slot of the
+        // item's first scales
+        uint32_t cur = 0, next = kStage, slot0 = 0;
+        // An item's outputs, through the stage `buf`: a lane's results are neighbours
         // of one row, but neighbouring lanes hold different rows, and stores of that
         // kind took 64 times a line each.  16-byte chunks are XOR-swizzled by their row.
         auto outputs = [&](auto &acc, uint32_t s, uint32_t buf) {
@@ -819,7 +823,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
                 for (int i = 0; i < NS; i++) {
                     const uint32_t row = 32 * i + 16 * tg + c, chunk = 2 * wg + (q >> 1);
                     const float r = q8_inverse(scale_of(row));
-                    *reinterpret_cast<u32x2q *>(lds.x[buf] + row * 128 + ((chunk ^ (row & 7)) << 4) + 8 * (q & 1)) =
+                    *reinterpret_cast<u32x2q *>(lds.x + buf + row * 128 + ((chunk ^ (row & 7)) << 4) + 8 * (q & 1)) =
                         u32x2q{q8_codes4(act[i][0], act[i][1], act[i][2], act[i][3], r),
                                q8_codes4(act[i][4], act[i][5], act[i][6], act[i][7], r)};
                 }
@@ -831,7 +835,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
                     const uint32_t row = 16 * wv + 8 * m + lane / 8, chunk = lane % 8, col = ct * 128 + 16 * chunk;
                     if (row < t.end - t.m0 && lds.map[s][row] != 0xffffffffu && col < a.out)
                         *reinterpret_cast<u32x4q *>(a.codes + (uint64_t)(t.m0 + row) * a.out + col) =
-                            *reinterpret_cast<const u32x4q *>(lds.x[buf] + row * 128 + ((chunk ^ (row & 7)) << 4));
+                            *reinterpret_cast<const u32x4q *>(lds.x + buf + row * 128 + ((chunk ^ (row & 7)) << 4));
                 }
             } else {
                 constexpr uint32_t B = MODE == F32OUT ? 4 : 2;              // bytes of a value
@@ -843,7 +847,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
                     store_rows<MODE, 4, NS>(a, acc, to, ct * 256 + wg * 64 + 16 * q);
                     return;
                 }
-                uint8_t *const mine = lds.w[buf] + 4096 * wv;  // of this wave alone
+                uint8_t *const mine = lds.w + 2 * buf + 4096 * wv;  // of this wave alone
 #pragma unroll
                 for (int h = 0; h < NS; h += P) {
 #pragma unroll
@@ -886,31 +890,32 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
             Codes wc[4], xc[NS];
             Scales sc;
 #pragma unroll
-            for (int j = 0; j < 4; j++) wc[j] = weights(stage, j);
+            for (int j = 0; j < 4; j++) wc[j] = weights(cur, j);
 #pragma unroll
-            for (int i = 0; i < NS; i++) xc[i] = tokens(stage, i);
-            grp = (grp + 1) % 4;
-            scales(sc, 0, grp);
-            auto step = [&](uint32_t kb, bool loads) {
-                stage = stage == kStages - 1 ? 0 : stage + 1;
+            for (int i = 0; i < NS; i++) xc[i] = tokens(cur, i);
+            scales(sc, slot0);
+            uint32_t slot = slot0 + 1;
+            // the step's loads go where its own rows were: they are read out
+            auto step = [&](bool loads, bool last) {
                 begin();
-                if (kb % kGroup == kGroup - 1) grp = (grp + 1) % 4;  // the next step's
-                compute(acc, wc, xc, sc, stage, kb, grp, loads, [&](uint32_t &lstage, uint32_t &lkb) {
-                    aim_next();
-                    lstage = pstage, lkb = pk;
-                    loaded();
+                compute(acc, wc, xc, sc, next, slot, last, [&](int i) {
+                    if (loads) load_part(i, cur);
                 });
+                slot = (slot + 1) % kScaleSlots;
+                cur = next;
+                next = next == 2 * kStage ? 0 : next + kStage;
             };
-            for (uint32_t kb = 0; kb + 1 < nk; kb++) step(kb, true);
-            // the buffer that the last step's loads would fill serves the outputs
-            // first: they leave through it in whole lines
-            step(nk - 1, false);
-            if (nk % kGroup == 0) grp = (grp + 3) % 4;  // (the last step looked past the item)
+            for (uint32_t kb = 0; kb + 1 < nk; kb++) step(true, false);
+            // where the last step's loads would go, the outputs are first: they
+            // leave through it in whole lines
+            const uint32_t spare = cur;
+            step(false, true);
+            slot0 = (slot0 + (nk + kGroup - 1) / kGroup * kGroup) % kScaleSlots;
             __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));
             landed = true;
-            outputs(acc, s, pstage);
+            outputs(acc, s, spare);
             barrier();
-            ahead();
+            ahead(spare);
         };
         for (uint32_t s = 0; s < slots; s++) {
             // (every wave takes the same way: the barriers are inside)
