@@ -598,7 +598,11 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
     const uint32_t dlocal = MODE == SWIGLU ? 8 * (dc >> 2) + 4 * (dj & 1) + (dc & 3) : 16 * (dc >> 2) + 4 * dj + (dc & 3);
     // the item whose steps are being loaded
     __amdgpu_buffer_rsrc_t rw = rx;
-    uint32_t xoff[NX] = {}, woff[NW] = {};
+    uint32_t xoff[NX] = {}, woff[NW] = {}, sxoff = 0, swoff = 0;
+    // the thread's share of the scales of kGroup steps: kSr neighbouring steps of one row
+    constexpr int kSr = kTileRows * kGroup / (64 * kTileWaves);
+    const uint32_t srow = tid / (kGroup / kSr), sk = tid % (kGroup / kSr) * kSr;
+    const bool has_sw = tid < 2 * kGroup;
     auto aim = [&](uint32_t s) {
         const Tile t = lds.slot[s];
         const uint32_t e = __builtin_amdgcn_readfirstlane(t.e);
@@ -609,12 +613,13 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
         for (int i = 0; i < NW; i++)
             woff[i] = min((MODE == SWIGLU ? t.ct * 128 + 32 * i : t.ct * 256 + 64 * i) + dlocal, a.out - 1) * a.in + dchunk;
         // positions past the item's end, and those that name no row, read some row
+        auto source = [&](uint32_t r) {
+            return MODE == SWIGLU ? min(lds.map[s][r], a.xrows - 1) : t.m0 + r < t.end ? t.m0 + r : t.m0;
+        };
 #pragma unroll
-        for (int i = 0; i < NX; i++) {
-            const uint32_t r = drow + 64 * i, p = t.m0 + r;
-            const uint32_t src = MODE == SWIGLU ? min(lds.map[s][r], a.xrows - 1) : p < t.end ? p : t.m0;
-            xoff[i] = src * a.in + dchunk;
-        }
+        for (int i = 0; i < NX; i++) xoff[i] = source(drow + 64 * i) * a.in + dchunk;
+        sxoff = source(srow) * nk;
+        swoff = (e * ob + (MODE == SWIGLU ? t.ct : min(2 * t.ct + tid / kGroup, ob - 1))) * nk;
     };
     // columns past `in` in the last step: a chunk is replaced by its row's first of
     // the block, and the weights' codes are zeroed when they are used
@@ -630,21 +635,13 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_ptr)(lds.w + 2 * to + (64 * (i - NX) + 8 * wv) * 128), 16,
                                                      woff[i < NX ? 0 : i - NX] - b, k, 0, 0);
     };
-    // the thread's share of the scales of kGroup steps: kSr neighbouring steps of one row
-    constexpr int kSr = kTileRows * kGroup / (64 * kTileWaves);
-    const uint32_t srow = tid / (kGroup / kSr), sk = tid % (kGroup / kSr) * kSr;
-    const bool has_sw = tid < 2 * kGroup;
     uint16_t sr[kSr];
     float swr = 0.f;
-    auto load_scales = [&](uint32_t s, uint32_t k0) {
-        const Tile t = lds.slot[s];
-        const uint32_t p = t.m0 + srow;
-        const uint32_t src = MODE == SWIGLU ? min(lds.map[s][srow], a.xrows - 1) : p < t.end ? p : t.m0;
+    auto load_scales = [&](uint32_t k0) {
 #pragma unroll
-        for (int i = 0; i < kSr; i++) sr[i] = a.xs[(uint64_t)src * nk + min(k0 + sk + i, nk - 1)];
-        const uint32_t b = MODE == SWIGLU ? t.ct : min(2 * t.ct + tid / kGroup, ob - 1);
+        for (int i = 0; i < kSr; i++) sr[i] = a.xs[sxoff + min(k0 + sk + i, nk - 1)];
         const void *from = MODE == SWIGLU && tid >= kGroup ? a.ws2 : a.ws;
-        if (has_sw) swr = scale_at(from, a.stype, ((uint64_t)t.e * ob + b) * nk + min(k0 + tid % kGroup, nk - 1));
+        if (has_sw) swr = scale_at(from, a.stype, swoff + min(k0 + tid % kGroup, nk - 1));
     };
     auto keep_scales = [&](uint32_t buf) {
 #pragma unroll
@@ -744,7 +741,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
             if (i == 0) {
                 if (due) {
                     if (pk == 0) aim(min(ps, slots - 1));
-                    load_scales(min(ps, slots - 1), pk / 128);
+                    load_scales(pk / 128);
                     pslot = (pslot + kGroup) % kScaleSlots;
                 }
                 pending = due;
@@ -992,12 +989,13 @@ static hipError_t launch_q8(Prof *p, hipStream_t s, const char *name, q8::Args a
     // and an expert's rows to be worth its steps (768 columns to 2048, 64 experts):
     //   bf16    512 rows: 21.6, 18.9;  1024: 21.9, 24.9      F32  512 rows: 24.4, 19.9;  1024: 24.8, 26.1
     // SwiGLU's steps are worth it from the first row on (2048 to 512, 512 experts: 640 rows 132, 144).
-    // DMA offsets are 32-bit.
+    // DMA offsets and the scales' indexes there are 32-bit.
     constexpr uint64_t kRows = MODE == SWIGLU ? 0 : MODE == F32OUT ? 16 : 12;
     const bool fills = ct * a.P >= (MODE == F32OUT ? 5120 : 2560) || (MODE == BF16OUT && ct * live >= 80) ||
                        (MODE == SWIGLU && ct * (a.P + 32 * live) >= 3520);
     const bool tiled = fills && a.P >= kRows * experts && (uint64_t)a.xrows * a.in < 0xffffffffull &&
-                       (uint64_t)a.out * a.in < 0xffffffffull;
+                       (uint64_t)a.out * a.in < 0xffffffffull &&
+                       (uint64_t)experts * ((a.out + 127) / 128) * a.kb < 0xffffffffull;
     // Two token tiles a wave read the weights half as often, where that leaves 256
     // waves (24 rows, 2048 columns to 4096: 5.1 us against 6.2; 4096 to 2048: 7.6 against 6.3)
     const bool two = a.P > 16ull * experts && (uint64_t)((a.out + 15) / 16) * ((a.P + 15) / 16) >= 512;
