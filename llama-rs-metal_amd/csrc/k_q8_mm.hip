@@ -552,7 +552,7 @@ __global__ __launch_bounds__(64 * NW, WPS) void stream_kernel(Args a) {
 // kSlots items.
 //
 // 4096 rows, 4096 columns to 12288, bf16: 200 us, 2060 TFLOP/s; 4001 rows, 2048 to
-// 4096: 39.5 us, 1700.  A step takes 1780 cycles: 1024 of matrix instructions; 768 of
+// 4096: 39.6 us, 1695.  A step takes 1750 cycles: 1024 of matrix instructions; 768 of
 // DMA at the 64 bytes a cycle a CU loads, which hold up the waves that issue them;
 // the scaling (64 FMA a wave) and reads of LDS fill the rest.  An item's first
 // loads and its outputs come to another 3500 cycles, the launch's to 7000.
