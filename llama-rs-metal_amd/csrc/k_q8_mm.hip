@@ -983,11 +983,11 @@ static hipError_t launch_q8(Prof *p, hipStream_t s, const char *name, q8::Args a
     //   SwiGLU  512 outputs, 1 expert, 512 rows (16 items): 19.1, 15.4;  4 experts, 1024 rows (32): 19.9, 46.3
     //           768 outputs, 16 experts, 16 rows (96 items): 15.2, 11.2;  128 rows: 15.6, 16.6;  256 rows: 15.5, 20.5
     //           512 outputs, 512 experts, 20 rows (80 items): 15.5, 14.6;  40 rows (160): 18.7, 22.9
-    //   bf16    4096 outputs, 128 rows (16 items): 16.8, 13.6;  256 rows (32): 17.3, 24.3
-    //           16384 outputs, 32 rows (64 items): 14.2, 13.8;  48 rows: 14.2, 24.4
-    //   F32     4096 outputs, 256 rows (32 items): 31.6, 25.4;  512 rows (64): 34.0, 38.3
+    //   bf16    4096 outputs, 128 rows (16 items): 16.0, 13.2;  256 rows (32): 16.4, 19.1
+    //           16384 outputs, 32 rows (64 items): 13.7, 13.6;  48 rows: 13.8, 19.4
+    //   F32     4096 outputs, 256 rows (32 items): 31.5, 20.3;  512 rows (64): 33.5, 38.3
     // and an expert's rows to be worth its steps (768 columns to 2048, 64 experts):
-    //   bf16    512 rows: 21.6, 18.9;  1024: 21.9, 24.9      F32  512 rows: 24.4, 19.9;  1024: 24.8, 26.1
+    //   bf16    512 rows: 21.3, 18.7;  1024: 21.7, 24.9      F32  512 rows: 23.5, 19.6;  1024: 24.1, 26.1
     // SwiGLU's steps are worth it from the first row on (2048 to 512, 512 experts: 640 rows 132, 144).
     // DMA offsets and the scales' indexes there are 32-bit.
     constexpr uint64_t kRows = MODE == SWIGLU ? 0 : MODE == F32OUT ? 16 : 12;
