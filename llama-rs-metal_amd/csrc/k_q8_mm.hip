@@ -103,7 +103,7 @@ __device__ __forceinline__ uint32_t find_items(const Args &a, uint32_t from, uin
         }
     }
     // (fewer than 2^31 items: the launch checks it.  Segments that overlap can make
-    // more tiles than the launch has blocks for: the last are left out, whole.)
+    // more tiles than the launch has blocks for: the last are left out.)
     total = min(total, a.tiles);
     const uint32_t items = total * a.col_tiles, range = (items + kXcds - 1) / kXcds;
     const uint32_t lo_item = blockIdx.x % kXcds * range, hi_item = min(items, lo_item + range);
@@ -111,7 +111,8 @@ __device__ __forceinline__ uint32_t find_items(const Args &a, uint32_t from, uin
     const uint32_t first = lo_item + blockIdx.x / kXcds + from * turn;
     if (first >= hi_item) return 0;
     const uint32_t n = min(kMax, (hi_item - first + turn - 1) / turn);
-    // item `i` of a segment of k tiles
+    // item `i` of a segment of k tiles, none of which `total` cuts off: a tile gets all of
+    // its columns or none (the counts of small SwiGLUs rely on it)
     auto put = [&](uint32_t s, uint32_t e, uint32_t lo, uint32_t hi, uint32_t k, uint32_t first_tile, uint32_t i) {
         const uint32_t panel = k < 2 * kPanel || a.col_tiles <= 2 * kPanel ? a.col_tiles : kPanel;
         const uint32_t ct = i / (k * panel) * panel;
@@ -131,7 +132,7 @@ __device__ __forceinline__ uint32_t find_items(const Args &a, uint32_t from, uin
                 uint32_t lo, k;
                 const uint32_t hi = seg(e0 + i, lo, k);
                 if (tile - at < k) {
-                    put(s, e0 + i, lo, hi, k, at, item - at * a.col_tiles);
+                    put(s, e0 + i, lo, hi, min(k, total - at), at, item - at * a.col_tiles);
                     break;
                 }
                 at += k;

@@ -547,6 +547,38 @@ def test_small_swiglu_over_and_over(gpu, own, T, n_in, ff, E):
     cap.graph.destroy()
 
 
+@pytest.mark.parametrize("T,n_in,ff", [(160, 2048, 512), (200, 1024, 512), (256, 1024, 512), (144, 1280, 528)])
+@pytest.mark.parametrize("perm", [False, True])
+def test_small_swiglu_after_more_tiles_than_a_launch_has(gpu, own, T, n_in, ff, perm):
+    """Two segments of all rows hold more tiles than the launch has blocks for, and
+    the cut falls inside a segment whose tiles go by panels of columns: each tile
+    runs whole or not at all, so that the next call finds the counts at zero."""
+    rng = np.random.default_rng(T + n_in)
+    w, w2 = Weight8(rng, 3, ff, n_in), Weight8(rng, 3, ff, n_in)
+    codes, bits = random_rows(rng, T, n_in)
+    wd, ud, x = own.weight(w.tensor()), own.weight(w2.tensor()), own.rows8(T, n_in, codes, bits)
+    offsets = [0, T // 3, T // 3, T]
+    ob, over = own.u32(offsets), own.u32([0, T, 0, T])
+    order = np.arange(T)
+    if perm:
+        order = rng.permutation(T)
+    pb = own.u32(order) if perm else None
+    many, spoilt = [own.rows8(T, ff) for _ in range(12)], own.rows8(T, ff)
+    with gpu.batch() as b:
+        for i, q in enumerate(many):
+            if i % 3 == 1:
+                b.expert_swiglu_q8(wd, ud, x, over, pb, 1, spoilt)
+            b.expert_swiglu_q8(wd, ud, x, ob, pb, 1, q)
+    v = rows_value(codes, bits)[order]
+    want, dw = (np.concatenate(p) for p in zip(*(swiglu64(v[a:c], w, w2, e)
+                                                for e, (a, c) in enumerate(zip(offsets[:-1], offsets[1:])))))
+    first = gpu.read_rows8(many[0])
+    check_quantized(*first, want, dw)
+    for q in many[1:]:
+        for i, j in zip(first, gpu.read_rows8(q)):
+            assert np.array_equal(i, j)
+
+
 def test_two_gpus_at_once(gpu, own):
     """Batches of two engines on one device, both in flight: neither sees the
     other's rows on their way to 8 bits in a small SwiGLU."""
