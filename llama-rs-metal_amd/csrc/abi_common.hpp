@@ -52,11 +52,9 @@ struct moe_gpu {
     hipEvent_t ev_fork = nullptr, ev_join = nullptr;
     // device word of the fused route + dispatch launch: zero between launches
     uint32_t *arrive = nullptr;
-    // F32 rows of a small moe_expert_swiglu_q8 on their way to 8 bits, and its
-    // blocks' counts: zero between launches (used on `stream` only, so calls and
-    // graph replays follow one another)
+    // F32 rows and tiles between the two launches of a small moe_expert_swiglu_q8
+    // (used on `stream` only, so calls and graph replays follow one another)
     float *q8_rows = nullptr;
-    uint32_t *q8_arrived = nullptr;
     // this device's copy of the no-allocation scratch array (moe_noalloc.cpp),
     // null when its address could not be obtained
     void *scratch = nullptr;

@@ -35,7 +35,7 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 
-enum { SWIGLU = 0, F32OUT = 1, BF16OUT = 2, ACT = 3 };  // ACT: SWIGLU whose blocks hold less than the 128 outputs of a scale
+enum { SWIGLU = 0, F32OUT = 1, BF16OUT = 2, ACT = 3 };  // ACT: SwiGLU as F32 rows
 
 struct Args {
     const uint8_t *w, *w2;        // codes (w2: the up weights of SWIGLU)
@@ -44,8 +44,8 @@ struct Args {
     const uint16_t *xs;           // and scales [xrows, kb]
     const uint32_t *offsets;      // [experts + 1], or null: one segment of all positions
     const uint32_t *perm;         // [P] pair of each position, or null: the position itself
-    void *y;                      // F32OUT / BF16OUT: [P, out]; ACT: F32 rows on the way
-    uint32_t *arrived;            // ACT: counts, zero between launches
+    void *y;                      // F32OUT / BF16OUT / ACT: [P, out]
+    uint32_t *list;               // ACT: the number of tiles, one word unused, first position and end of each
     uint8_t *codes;               // SWIGLU: [P, out] and scales [P, ceil(out / 128)]
     uint16_t *scales;
     uint32_t stype, xrows, in, out, kb, experts, P, kdiv;
@@ -63,14 +63,14 @@ struct Args {
 // 4096 to 12288 columns: 200 us; 205 with panels of 8, 224 of 1, 247 of all).
 // Every thread of the block calls it; slots `from` and on of the block are written to out[0 .. n), at most
 // kMax; n is returned.  Offsets past P count as P and a segment that ends before
-// it starts is empty.
+// it starts is empty.  `list`: where the launch leaves its tiles, for the next one.
 struct Tile {
     uint32_t e, m0, end, ct;
 };
 constexpr uint32_t kXcds = 8, kPanel = 4;
 template <int BM, int NW>
 __device__ __forceinline__ uint32_t find_items(const Args &a, uint32_t from, uint32_t kMax, Tile *out, uint32_t *lds /* NW */,
-                                               uint32_t *number = nullptr) {
+                                               uint32_t *list = nullptr) {
     const uint32_t tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     const uint32_t per = (a.experts + 64 * NW - 1) / (64 * NW), e0 = tid * per;
     auto seg = [&](uint32_t e, uint32_t &lo, uint32_t &n) {
@@ -105,6 +105,7 @@ __device__ __forceinline__ uint32_t find_items(const Args &a, uint32_t from, uin
     // (fewer than 2^31 items: the launch checks it.  Segments that overlap can make
     // more tiles than the launch has blocks for: the last are left out.)
     total = min(total, a.tiles);
+    if (list && blockIdx.x == 0 && tid == 0) list[0] = total;
     const uint32_t items = total * a.col_tiles, range = (items + kXcds - 1) / kXcds;
     const uint32_t lo_item = blockIdx.x % kXcds * range, hi_item = min(items, lo_item + range);
     const uint32_t turn = gridDim.x / kXcds;
@@ -112,14 +113,17 @@ __device__ __forceinline__ uint32_t find_items(const Args &a, uint32_t from, uin
     if (first >= hi_item) return 0;
     const uint32_t n = min(kMax, (hi_item - first + turn - 1) / turn);
     // item `i` of a segment of k tiles, none of which `total` cuts off: a tile gets all of
-    // its columns or none (the counts of small SwiGLUs rely on it)
+    // its columns or none
     auto put = [&](uint32_t s, uint32_t e, uint32_t lo, uint32_t hi, uint32_t k, uint32_t first_tile, uint32_t i) {
         const uint32_t panel = k < 2 * kPanel || a.col_tiles <= 2 * kPanel ? a.col_tiles : kPanel;
         const uint32_t ct = i / (k * panel) * panel;
         const uint32_t wide = min(panel, a.col_tiles - ct), at = i - k * ct;
-        const uint32_t m0 = lo + at / wide * BM;
-        if (number) *number = first_tile + at / wide;
-        out[s] = Tile{e, m0, hi - m0 < BM ? hi : m0 + BM, ct + at % wide};
+        const uint32_t m0 = lo + at / wide * BM, end = hi - m0 < BM ? hi : m0 + BM;
+        out[s] = Tile{e, m0, end, ct + at % wide};
+        if (list && ct + at % wide == 0) {
+            uint32_t *const l = list + 2 + 2 * (first_tile + at / wide);
+            l[0] = m0, l[1] = end;
+        }
     };
     if (!a.offsets) {
         if (tid < n) put(tid, 0, 0, a.P, total, 0, first + tid * turn);
@@ -143,13 +147,12 @@ __device__ __forceinline__ uint32_t find_items(const Args &a, uint32_t from, uin
     return n;
 }
 // The one item of a block in a grid with a block per item.
-constexpr int kFind = 13;  // its words of LDS
+constexpr int kFind = 12;  // its words of LDS
 template <int BM, int NW>
-__device__ __forceinline__ bool find_tile(const Args &a, Tile &t, uint32_t &number, uint32_t *lds) {
-    static_assert(NW + 5 <= kFind, "LDS words");
+__device__ __forceinline__ bool find_tile(const Args &a, Tile &t, uint32_t *lds, uint32_t *list) {
+    static_assert(NW + 4 <= kFind, "LDS words");
     Tile *out = reinterpret_cast<Tile *>(lds + NW);
-    if (find_items<BM, NW>(a, 0, 1, out, lds, lds + NW + 4) == 0) return false;
-    number = __builtin_amdgcn_readfirstlane(lds[NW + 4]);
+    if (find_items<BM, NW>(a, 0, 1, out, lds, list) == 0) return false;
     t.e = __builtin_amdgcn_readfirstlane(out->e);
     t.m0 = __builtin_amdgcn_readfirstlane(out->m0);
     t.end = __builtin_amdgcn_readfirstlane(out->end);
@@ -308,17 +311,6 @@ __device__ __forceinline__ void store_swiglu(const Args &a, const f32x4q (&acc)[
     }
 }
 
-// Two values, 8-byte aligned, to and from what every XCD sees.
-__device__ __forceinline__ void store_agent(float *p, float a, float b) {
-    const uint64_t v = (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
-    __hip_atomic_store(reinterpret_cast<uint64_t *>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ void load_agent(const float *p, float &a, float &b) {
-    const uint64_t v =
-        __hip_atomic_load(reinterpret_cast<const uint64_t *>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    a = __uint_as_float((uint32_t)v), b = __uint_as_float((uint32_t)(v >> 32));
-}
-
 // Few rows per expert: the time is the weights' way from memory, so what counts
 // is how many of their loads are in flight.  A wave owns RT row tiles (SWIGLU: 16
 // gate rows and their up rows) and a range of the blocks of 128 columns (KS waves
@@ -356,8 +348,7 @@ __global__ __launch_bounds__(64 * NW, WPS) void stream_kernel(Args a) {
     static_assert(RG * kCols <= 128 && 128 % (RG * kCols) == 0, "a block's rows share their scales");
     __shared__ __attribute__((aligned(16))) StreamLds<MODE, RT, TT, KS, NW> lds;
     Tile t;
-    uint32_t number;
-    if (!find_tile<BM, NW>(a, t, number, lds.find)) return;
+    if (!find_tile<BM, NW>(a, t, lds.find, MODE == ACT ? a.list : nullptr)) return;
     const uint32_t tid = threadIdx.x, lane = tid & 63, c = lane & 15, q = lane >> 4;
     const uint32_t wv = __builtin_amdgcn_readfirstlane(tid >> 6), rg = wv / KS, ks = wv % KS;
     const uint32_t n0 = t.ct * (RG * kCols) + rg * kCols, nb = min(n0, a.out - 1);
@@ -473,67 +464,26 @@ __global__ __launch_bounds__(64 * NW, WPS) void stream_kernel(Args a) {
                     *reinterpret_cast<f32x4q *>(r + ((j * TT + i) * 64 + lane) * 4) = acc[j][i];
         }
         __syncthreads();
-        if (MODE != ACT && ks > 0) return;
+        if (ks > 0) return;
 #pragma unroll
         for (int v = 0; v < KS - 1; v++)
 #pragma unroll
             for (int j = 0; j < RT; j++)
 #pragma unroll
                 for (int i = 0; i < TT; i++)
-                    if (ks == 0) acc[j][i] += *reinterpret_cast<const f32x4q *>(lds.red[rg * (KS - 1) + v] + ((j * TT + i) * 64 + lane) * 4);
+                    acc[j][i] += *reinterpret_cast<const f32x4q *>(lds.red[rg * (KS - 1) + v] + ((j * TT + i) * 64 + lane) * 4);
     }
     if constexpr (MODE == SWIGLU)
         store_swiglu<RT, TT, NW>(a, acc, to, n0 + 4 * q, t.ct, wv, lds.tops);
     else if constexpr (MODE == ACT) {
-        // The block's outputs as F32 rows; the last block of the 128 that share a
-        // scale quantises them.  The rows are stored and loaded past the caches of
-        // one XCD (agent scope) and the stores have landed (vmcnt) before the count:
-        // fences, which write back and drop a whole L2, took 30 us here.
-        float *const rows = static_cast<float *>(a.y);
+        if (n0 + 4 * q >= a.out) return;  // (out is a multiple of 16)
 #pragma unroll
         for (int i = 0; i < TT; i++) {
-            if (ks > 0 || to[i] == 0xffffffffu || n0 + 4 * q >= a.out) continue;  // (out is a multiple of 16)
+            if (to[i] == 0xffffffffu) continue;
             f32x4q v;
 #pragma unroll
             for (int e = 0; e < 4; e++) v[e] = swiglu_of(acc[0][i][e], acc[1][i][e]);
-            float *const at = rows + (uint64_t)to[i] * a.out + n0 + 4 * q;
-            store_agent(at, v[0], v[1]);
-            store_agent(at + 2, v[2], v[3]);
-        }
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(0);
-        __syncthreads();
-        constexpr uint32_t kOuts = RG * kCols;  // outputs of a block
-        const uint32_t group = t.ct * kOuts / 128, cols = min(128u, a.out - 128 * group);
-        if (tid == 0) {
-            uint32_t *const count = a.arrived + number * ob + group;
-            const bool last = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
-                              (cols + kOuts - 1) / kOuts - 1;
-            if (last) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            lds.find[0] = last;
-        }
-        __syncthreads();
-        if (!lds.find[0]) return;
-        // 16 lanes hold the columns of a row, eight each
-#pragma unroll
-        for (int r = 0; r < BM; r += 4 * NW) {
-            const uint32_t p = t.m0 + r + tid / 16, col = tid % 16 * 8;
-            const bool row = p < t.end && (a.perm ? a.perm[p] : p) / a.kdiv < a.xrows, live = row && col < cols;
-            const float *const from = rows + (uint64_t)p * a.out + 128 * group + col;
-            float v[8] = {};
-            if (live) {
-#pragma unroll
-                for (int j = 0; j < 8; j += 2) load_agent(from + j, v[j], v[j + 1]);
-            }
-            uint32_t top = 0;
-#pragma unroll
-            for (int j = 0; j < 8; j++) top = max(top, abs_word(v[j]));
-            const uint32_t sb = q8_scale_bits(row16_max(top));
-            if (!live) continue;
-            const float inv = q8_inverse(sb);
-            *reinterpret_cast<u32x2q *>(a.codes + (uint64_t)p * a.out + 128 * group + col) =
-                u32x2q{q8_codes4(v[0], v[1], v[2], v[3], inv), q8_codes4(v[4], v[5], v[6], v[7], inv)};
-            if (col == 0) a.scales[(uint64_t)p * ob + group] = (uint16_t)sb;
+            *reinterpret_cast<f32x4q *>(static_cast<float *>(a.y) + (uint64_t)to[i] * a.out + n0 + 4 * q) = v;
         }
     } else
         store_rows<MODE, RT, TT>(a, acc, to, n0 + 4 * RT * q);
@@ -929,6 +879,34 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
     }
 }
 
+// ACT's F32 rows in 8 bits, tile by tile as its launch listed them: a block per tile
+// and 128 columns, whose 16 lanes hold eight columns of a row each.
+constexpr int kQuantThreads = 256;
+__global__ __launch_bounds__(kQuantThreads) void quantize_kernel(Args a) {
+    const uint32_t tid = threadIdx.x, ob = gridDim.y, col = 128 * blockIdx.y + 8 * (tid % 16);
+    const uint32_t m0 = a.list[2 + 2 * blockIdx.x], end = a.list[3 + 2 * blockIdx.x];
+    if (blockIdx.x >= a.list[0]) return;
+    const bool cols_in = col < a.out;  // (out is a multiple of 16)
+    for (uint32_t p = m0 + tid / 16; p < end; p += kQuantThreads / 16) {
+        float v[8] = {};
+        if (cols_in) {
+            const float *const from = static_cast<const float *>(a.y) + (uint64_t)p * a.out + col;
+            const f32x4q lo = *reinterpret_cast<const f32x4q *>(from), hi = *reinterpret_cast<const f32x4q *>(from + 4);
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = lo[j], v[4 + j] = hi[j];
+        }
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) top = max(top, abs_word(v[j]));
+        const uint32_t sb = q8_scale_bits(row16_max(top));
+        if (!cols_in || (a.perm ? a.perm[p] : p) / a.kdiv >= a.xrows) continue;
+        const float r = q8_inverse(sb);
+        *reinterpret_cast<u32x2q *>(a.codes + (uint64_t)p * a.out + col) =
+            u32x2q{q8_codes4(v[0], v[1], v[2], v[3], r), q8_codes4(v[4], v[5], v[6], v[7], r)};
+        if (tid % 16 == 0) a.scales[(uint64_t)p * ob + blockIdx.y] = (uint16_t)sb;
+    }
+}
+
 }  // namespace q8
 
 // The stream kernel's forms of one mode: its outputs per block and its kernel.
@@ -1006,11 +984,19 @@ static hipError_t launch_q8(Prof *p, hipStream_t s, const char *name, q8::Args a
     const uint64_t tiles = max_tiles(two ? 32 : 16);
     if constexpr (MODE == SWIGLU) {
         // A scale needs 128 outputs: blocks that hold them (512 KiB of weights at
-        // 2048 columns) are few, so blocks of 16 to 64 write F32 rows and the last
-        // of each 128 quantises them.  (What does not fit has 2^32 bytes of rows or weights.)
-        if ((uint64_t)a.P * a.out <= kQ8RowsLen && tiles * ((a.out + 127) / 128) <= kQ8CountLen)
-            return launch_form(p, s, name, two ? stream_form<ACT, 2>(a.out, a.kb, tiles) : stream_form<ACT, 1>(a.out, a.kb, tiles),
-                               tiles, a);
+        // 2048 columns) are few, so blocks of 16 to 64 write F32 rows and a second
+        // launch quantises them (10 rows of 512 experts: 20.2 us, 12.3).  One launch
+        // whose last block of each 128 quantises took 11.1 where the rows' order
+        // rested on their stores having landed; 14.2 with a release and an acquire
+        // around the count, which write back and drop a whole L2.  (What does not
+        // fit has 2^32 bytes of rows or weights.)
+        if ((uint64_t)a.P * a.out <= kQ8RowsLen && tiles <= kQ8TilesLen) {
+            const hipError_t e = launch_form(
+                p, s, name, two ? stream_form<ACT, 2>(a.out, a.kb, tiles) : stream_form<ACT, 1>(a.out, a.kb, tiles), tiles, a);
+            if (e != hipSuccess) return e;
+            return launch_kernel(p, "quantize_q8", quantize_kernel, dim3((uint32_t)tiles, (a.out + 127) / 128),
+                                 dim3(kQuantThreads), 0, s, a);
+        }
         return launch_form(p, s, name, stream_form<SWIGLU, 1>(a.out, a.kb, max_tiles(16)), max_tiles(16), a);
     } else {
         return launch_form(p, s, name, two ? stream_form<MODE, 2>(a.out, a.kb, tiles) : stream_form<MODE, 1>(a.out, a.kb, tiles),
@@ -1029,14 +1015,14 @@ hipError_t launch_q8_rows(Prof *p, hipStream_t s, const char *name, const Q8Weig
 
 hipError_t launch_q8_swiglu(Prof *p, hipStream_t s, const Q8Weight &gate, const Q8Weight &up, const Q8Rows &x,
                             const uint32_t *offsets, const uint32_t *perm, uint32_t k, const Q8Rows &out,
-                            float *rows, uint32_t *arrived) {
+                            float *rows) {
     q8::Args a{};
     a.w = gate.codes, a.ws = gate.scales, a.w2 = up.codes, a.ws2 = up.scales, a.stype = gate.stype;
     a.in = gate.in, a.out = gate.out, a.experts = gate.experts;
     a.x = x.codes, a.xs = x.scales, a.xrows = x.rows, a.P = out.rows;
     a.offsets = offsets, a.perm = perm, a.kdiv = k;
     a.codes = out.codes, a.scales = out.scales;
-    a.y = rows, a.arrived = arrived;
+    a.y = rows, a.list = reinterpret_cast<uint32_t *>(rows + kQ8RowsLen);
     return launch_q8<q8::SWIGLU>(p, s, "expert_swiglu_q8", a);
 }
 

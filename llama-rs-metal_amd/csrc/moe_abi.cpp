@@ -82,11 +82,8 @@ moe_status moe_gpu_create(int device, moe_gpu **out) {
         hipEventCreateWithFlags(&g->ev_join, hipEventDisableTiming) != hipSuccess ||
         hipMalloc(reinterpret_cast<void **>(&g->arrive), 256) != hipSuccess ||
         zero_new(g, g->arrive, 256) != hipSuccess ||
-        hipMalloc(reinterpret_cast<void **>(&g->q8_rows), kQ8RowsLen * 4) != hipSuccess ||
-        hipMalloc(reinterpret_cast<void **>(&g->q8_arrived), kQ8CountLen * 4) != hipSuccess ||
-        zero_new(g, g->q8_arrived, kQ8CountLen * 4) != hipSuccess) {
-        for (void *p : {(void *)g->arrive, (void *)g->q8_rows, (void *)g->q8_arrived})
-            if (p) (void)hipFree(p);
+        hipMalloc(reinterpret_cast<void **>(&g->q8_rows), kQ8SpaceLen * 4) != hipSuccess) {
+        if (g->arrive) (void)hipFree(g->arrive);
         delete g;
         return MOE_ERR_GPU;
     }
@@ -111,7 +108,6 @@ void moe_gpu_destroy(moe_gpu *g) {
     for (auto e : g->prof.pool) (void)hipEventDestroy(e);
     (void)hipFree(g->arrive);
     (void)hipFree(g->q8_rows);
-    (void)hipFree(g->q8_arrived);
     (void)hipEventDestroy(g->ev_begin);
     (void)hipEventDestroy(g->ev_end);
     (void)hipEventDestroy(g->ev_fork);

@@ -283,12 +283,14 @@ hipError_t launch_mix_tokens(Prof *p, hipStream_t s, const void *x, bool bf16, c
 hipError_t launch_q8_rows(Prof *p, hipStream_t s, const char *name, const Q8Weight &w, const Q8Rows &x,
                           const uint32_t *offsets, const uint32_t *perm, void *y, bool bf16);
 // out[p] = silu(x_t . G_e) * (x_t . U_e), t = perm[p] / k (perm null: p);
-// rows, arrived: an engine's kQ8RowsLen floats and kQ8CountLen counts, zero between
-// launches, for few positions
-constexpr uint64_t kQ8RowsLen = 2560 * 128, kQ8CountLen = 22528;
+// rows: an engine's kQ8SpaceLen words, for few positions: F32 rows of kQ8RowsLen
+// values and a list of kQ8TilesLen tiles (with fewer than 2560 positions times
+// blocks of 128 outputs, and 3520 with 32 more positions for each segment, there
+// are at most P / 16 + (3520 - P) / 32 < 190 tiles)
+constexpr uint64_t kQ8RowsLen = 2560 * 128, kQ8TilesLen = 256, kQ8SpaceLen = kQ8RowsLen + 2 + 2 * kQ8TilesLen;
 hipError_t launch_q8_swiglu(Prof *p, hipStream_t s, const Q8Weight &gate, const Q8Weight &up, const Q8Rows &x,
                             const uint32_t *offsets, const uint32_t *perm, uint32_t k, const Q8Rows &out,
-                            float *rows, uint32_t *arrived);
+                            float *rows);
 
 // ---- fused single-token decode (k_decode.hip) ----
 struct DecodeArgs {

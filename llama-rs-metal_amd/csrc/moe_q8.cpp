@@ -1,5 +1,5 @@
 // C entries of the 8-bit floating point operators (include/moe_hip.h): checks,
-// then one launch each.  No counterpart in the reference, whose weights are
+// then one launch each (two for a SwiGLU of few positions).  No counterpart in the reference, whose weights are
 // affine, GGML or dense.
 #include "abi_common.hpp"
 
@@ -165,7 +165,7 @@ moe_status moe_expert_swiglu_q8(moe_gpu *g, const moe_weight *gate, const moe_we
     return launched(g, launch_q8_swiglu(&g->prof, g->stream, q8_weight(*gate), q8_weight(*up), q8_rows(x),
                                         (const uint32_t *)offsets.ptr,
                                         has(perm) ? (const uint32_t *)perm.ptr : nullptr, (uint32_t)k, q8_rows(q),
-                                        g->q8_rows, g->q8_arrived),
+                                        g->q8_rows),
                     "expert_swiglu_q8");
 }
 
