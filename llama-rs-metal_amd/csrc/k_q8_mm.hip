@@ -84,13 +84,13 @@ __device__ __forceinline__ uint32_t find_items(const Args &a, uint32_t from, uin
         for (uint32_t i = 0; i < per && e0 + i < a.experts; i++) {
             uint32_t lo, n;
             seg(e0 + i, lo, n);
-            mine += n;
+            mine = min(mine + n, a.tiles);
         }
         uint32_t incl = mine;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
             const uint32_t up = __shfl_up(incl, d);
-            if ((int)lane >= d) incl += up;
+            if ((int)lane >= d) incl = __builtin_elementwise_add_sat(incl, up);
         }
         if (lane == 63) lds[wv] = incl;
         __syncthreads();
@@ -98,12 +98,13 @@ __device__ __forceinline__ uint32_t find_items(const Args &a, uint32_t from, uin
         total = 0;
 #pragma unroll
         for (uint32_t v = 0; v < NW; v++) {
-            if (v < wv) before += lds[v];
-            total += lds[v];
+            if (v < wv) before = __builtin_elementwise_add_sat(before, lds[v]);
+            total = __builtin_elementwise_add_sat(total, lds[v]);
         }
     }
     // (fewer than 2^31 items: the launch checks it.  Segments that overlap can make
-    // more tiles than the launch has blocks for: the last are left out.)
+    // more tiles than the launch has blocks for, and than 32 bits count: sums stop at
+    // 2^32 - 1 and a thread's tiles at a.tiles, the last tiles are left out.)
     total = min(total, a.tiles);
     if (list && blockIdx.x == 0 && tid == 0) list[0] = total;
     const uint32_t items = total * a.col_tiles, range = (items + kXcds - 1) / kXcds;

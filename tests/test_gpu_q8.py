@@ -579,6 +579,19 @@ def test_small_swiglu_after_more_tiles_than_a_launch_has(gpu, own, T, n_in, ff, 
             assert np.array_equal(i, j)
 
 
+def test_more_tiles_than_32_bits_count(gpu, own):
+    """8192 segments of all rows, 2^32 + 8192 tiles of 128: those of the first
+    segments run, and with them every row has its product."""
+    E, P, n_in, out = 16384, (1 << 26) + 128, 16, 2
+    w = Weight8(np.random.default_rng(3), E, out, n_in)
+    wd, x, y = own.weight(w.tensor()), own.rows8(P, n_in), own.zeros(P * out // 2)
+    gpu.write(y, np.full(P * out // 2, 0x55555555, np.uint32).view(np.float32))
+    ob = own.u32(np.arange(E + 1) % 2 * P)
+    with gpu.batch() as b:
+        b.expert_matmul_q8(wd, x, ob, None, y, BF16)
+    assert not gpu.read_u32(y).any()
+
+
 def test_two_gpus_at_once(gpu, own):
     """Batches of two engines on one device, both in flight: neither sees the
     other's rows on their way to 8 bits in a small SwiGLU."""
