@@ -334,7 +334,8 @@ moe_status moe_block_noalloc(moe_gpu *gpu, const moe_block_weights *w, moe_buffe
 /* Rows in 8 bits: codes [rows, n], n a multiple of 16, 16-byte aligned, and one
  * BF16 scale per row and 128 columns, [rows, ceil(n/128)].  Quantised here:
  * scale = bf16(max(max|v| / 448, 2^-126)), code = e4m3(v / scale), each to
- * nearest even.  128 columns that hold an infinity or a NaN read back as NaN. */
+ * nearest even, the quotients in F32 (moe_expert_swiglu_q8: v / scale within
+ * 2^-22 of it).  128 columns that hold an infinity or a NaN read back as NaN. */
 typedef struct {
     moe_region codes;
     moe_region scales;

@@ -9,12 +9,14 @@ namespace moehip {
 //
 // One block per row; a thread holds groups of eight columns, so 16 lanes (one
 // DPP row) hold the 128 columns that share a scale.  Rows of up to
-// kNormHold * 2048 columns are read once and stay in registers between the sum
+// kQ8NormHold * 2048 columns are read once and stay in registers between the sum
 // of squares and the output; longer ones are read again (as s, from `sum`
 // where that is written: it may be x or the residual itself).
 //
 // Bound by its bytes: 4096 rows of 2048 with residual, sum and F32 rows, 143 MB in
-// 33.5 us or 4.3 TB/s, where a copy reaches 4.65; one row takes an empty launch's 4 us.
+// 33.9 us or 4.2 TB/s, where a copy reaches 4.65; one row takes an empty launch's 4 us.
+// (`y` shows v, so its codes are those of the true F32 quotient: divisions, 33.9 us,
+// where products with a reciprocal took 33.8 and missed quotients between two codes.)
 constexpr uint32_t kQ8NormThreads = 256, kQ8NormHold = 2;
 
 template <int T, bool VEC>
@@ -84,11 +86,13 @@ __global__ __launch_bounds__(kQ8NormThreads) void norm_q8_kernel(const float *x,
         }
         top = row16_max(top);
         const uint32_t sb = q8_scale_bits(top);
-        const float r = q8_inverse(sb);
+        const float scale = bf16_to_f32(sb);
         if (!live) return;
         if (y) store(y, i, o);
+#pragma unroll
+        for (int j = 0; j < 8; j++) o[j] /= scale;
         *reinterpret_cast<u32x2q *>(codes + base + i) =
-            u32x2q{q8_codes4(o[0], o[1], o[2], o[3], r), q8_codes4(o[4], o[5], o[6], o[7], r)};
+            u32x2q{q8_codes4(o[0], o[1], o[2], o[3]), q8_codes4(o[4], o[5], o[6], o[7])};
         if ((tid & 15) == 0) scales[(uint64_t)row * nb + i / 128] = (uint16_t)sb;
     };
 #pragma unroll

@@ -44,11 +44,16 @@ __device__ __forceinline__ uint32_t q8_scale_bits(uint32_t top) {
 }
 // 1 / scale, within 2^-23 of it (a scale is at least 2^-126)
 __device__ __forceinline__ float q8_inverse(uint32_t sb) { return __builtin_amdgcn_rcpf(bf16_to_f32(sb)); }
-// Four values as e4m3 codes (nearest even; r: 1 / scale).  |v| * r is at most
+// Four quotients v / scale as e4m3 codes (nearest even).  They are at most
 // 448 * (1 + 2^-8), which rounds to 448.
+__device__ __forceinline__ uint32_t q8_codes4(float a, float b, float c, float d) {
+    int v = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, v, true);
+}
+// Four values, r = 1 / scale: each product is within 2^-22 of the quotient.  For
+// values that are seen in 8 bits only, and are further off than that themselves.
 __device__ __forceinline__ uint32_t q8_codes4(float a, float b, float c, float d, float r) {
-    int v = __builtin_amdgcn_cvt_pk_fp8_f32(a * r, b * r, 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c * r, d * r, v, true);
+    return q8_codes4(a * r, b * r, c * r, d * r);
 }
 
 }  // namespace moehip

@@ -3,7 +3,7 @@ points, against their 64-bit forms (helpers_q8)."""
 import numpy as np
 import pytest
 
-from helpers_q8 import (U, Weight8, bf16, check_quantized, cut_bound, decode, encode, f32_bound, nblocks, product,
+from helpers_q8 import (POS, U, Weight8, bf16, check_quantized, cut_bound, decode, encode, f32_bound, nblocks, product,
                         quantize_rows, random_rows, rows_value, silu, spread)
 from hip_backend import BF16, E4M3, F16, F32, Batch, Buffer, Gpu, Rows8, ShapeError, Tensor
 from hip_backend.api import MoeBufferC, MoeRegionC
@@ -162,6 +162,34 @@ def test_norm_q8_of_zeros_tiny_and_non_finite_rows(gpu, own):
     assert np.isnan(v[2, :128]).all()                  # inf * 0
     want = norm64(x[4:], w.astype(np.float64), 1e-6)
     check_quantized(codes[4:], bits[4:], want, 70 * U * np.abs(want) + 2.0 ** -149)
+
+
+@pytest.mark.parametrize("least", [False, True])
+def test_norm_q8_codes_of_quotients_between_two_codes(gpu, own, least):
+    """Rows of ones and minus ones have the norm's weights as their values: those
+    are each middle between two codes times each mantissa of a scale, and the
+    F32 values next to it.  The codes are those of the quotient in F32."""
+    mids = (POS[:-1] + POS[1:]) / 2
+    scales = np.array([2.0 ** -126] if least else (1 + np.arange(128) / 128) * 2.0 ** -9)
+    exact = np.zeros((len(scales), 128), np.float32)
+    exact[:, 0] = 448 * scales
+    exact[:, 1:127] = scales[:, None] * mids
+    assert np.array_equal(exact[:, 1:127].astype(np.float64), scales[:, None] * mids)
+    x = np.where(np.arange(exact.size) % 3 == 1, -1, 1).astype(np.float32)
+    for w in (exact, np.nextafter(exact, np.float32(0)), np.nextafter(exact, np.float32(np.inf))):
+        w = w.copy()
+        w[:, 0] = exact[:, 0]
+        for part in (w.ravel(), w.ravel()[:min(w.size, 2048)]):   # a long row; one that stays in registers
+            n = part.size
+            wd, xb, y, q = own.weight(Tensor.dense([n], part)), own.upload(x[:n]), own.zeros(n), own.rows8(1, n)
+            with gpu.batch() as b:
+                b.norm_q8(xb, None, wd, None, y, q, 1e-30)
+            v = gpu.read(y)
+            assert np.array_equal(v, x[:n] * part)
+            codes, bits = gpu.read_rows8(q)
+            s = spread(bf16(bits[0]), n)
+            assert np.array_equal(s, spread(scales, n).astype(np.float32))
+            assert np.array_equal(codes[0], encode((v / s).astype(np.float64)))
 
 
 # ------------------------------------------------------------------ dense --
