@@ -311,6 +311,8 @@ class Bound:
                 self.w = self.weight(s["w8"], s["ws"], [ff, h, E], "f32")
                 self.out = torch.empty(P, h, dtype=TYPES[s["y"]], device="cuda")
                 self.y, self.ytype = self.buffer(self.out), hb.F32 if s["y"] == "f32" else hb.BF16
+        # the engine's stream does not wait for torch's, which makes the inputs
+        torch.cuda.current_stream().synchronize()
 
     def adopt(self, t):
         lib = self.hb.load_library()
@@ -356,11 +358,18 @@ class Bound:
         return hb.Weight(c, [c.data], dims, 0)
 
     def drop(self):
-        lib = self.hb.load_library()
-        self.kept = [t for t in self.kept if lib.moe_unregister(self.gpu._h, ctypes.c_void_p(t.data_ptr())) != 0]
+        """Takes the tensors back when no pass is left that reads or writes them."""
+        try:
+            torch.cuda.synchronize()
+            lib = self.hb.load_library()
+            self.kept = [t for t in self.kept if lib.moe_unregister(self.gpu._h, ctypes.c_void_p(t.data_ptr())) != 0]
+        except (TypeError, AttributeError):
+            pass  # the interpreter is ending: its modules and the engine are gone
 
 
 def own_run(s):
+    """The calls go to the engine's own stream: who reads their outputs with torch
+    waits for the device first."""
     if s.bound is None:
         s.bound = Bound(s)
     b, o = s.bound.batch, s.bound
