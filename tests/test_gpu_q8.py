@@ -455,6 +455,181 @@ def test_expert_swiglu_q8_of_many_rows(gpu, own, lens, n_in, ff):
             check_quantized(got[a:b_], gs[a:b_], *swiglu64(v[a:b_], gate, up, e))
 
 
+SKIPS = [
+    lambda P: ([0, P // 6, P // 6, P // 4 * 3], None),                           # positions behind the last segment
+    lambda P: ([0, P // 4, P // 3 * 2, 4 * P], None),                            # an end past the positions
+    lambda P: ([P // 10, P // 10 + 1, P - 1, P - 1], None),                      # before the first one
+    lambda P: ([P // 4, P // 2, P // 5, P // 5 * 2], (P // 4, P // 5 * 2)),      # an end before its start, an overlap
+    lambda P: ([P + 10, 2 * P, 3 * P, 4000000000], None),                        # none
+]
+
+
+@pytest.mark.parametrize("skip", range(len(SKIPS)))
+@pytest.mark.parametrize("P,n_in,out,K", [(60, 272, 272, 2), (3000, 272, 272, 1), (3000, 128, 144, 2), (6000, 144, 130, 1)])
+def test_rows_left_as_they_were_in_every_form(gpu, own, P, n_in, out, K, skip):
+    """Segments that leave positions out and perms that name no row, over few rows
+    and in tiles of 128: what no position names keeps what it held, the rest is
+    its product."""
+    rng = np.random.default_rng(P + n_in + skip)
+    offsets, twice = SKIPS[skip](P)
+    E = len(offsets) - 1
+    gate, up, down = (Weight8(rng, E, out, n_in) for _ in range(3))
+    perm = rng.permutation(P).astype(np.uint32)
+    named = np.ones(P, bool)
+    for i, at in enumerate((0, P // 8, P // 4, P // 3, P - 1)):
+        perm[at], named[at] = (P, 0xFFFFFFFF, P + 1)[i % 3], False
+    inside, expert = np.zeros(P, bool), np.zeros(P, np.int64)
+    for e in range(E):
+        inside[offsets[e]:offsets[e + 1]] = True
+        expert[offsets[e]:offsets[e + 1]] = e
+    written, sure = inside & named, inside & named
+    if twice:                                   # rows of two segments: of either
+        sure = sure.copy()
+        sure[twice[0]:twice[1]] = False
+    ob, pb = own.u32(np.array(offsets, np.uint32)), own.u32(perm)
+    if out % 16 == 0:
+        gd, ud = own.weight(gate.tensor()), own.weight(up.tensor())
+        codes, bits = random_rows(rng, P // K, n_in)
+        x = own.rows8(P // K, n_in, codes, bits)
+        q = own.rows8(P, out, np.full((P, out), 0x55, np.uint8), np.full((P, nblocks(out)), 0x1234, np.uint16))
+        with gpu.batch() as b:
+            b.expert_swiglu_q8(gd, ud, x, ob, pb, K, q)
+        c, s = gpu.read_rows8(q)
+        assert np.all(c[~written] == 0x55) and np.all(s[~written] == 0x1234) and not np.any(s[written] == 0x1234)
+        for e in range(E):
+            at = np.flatnonzero(sure & (expert == e))
+            if at.size:
+                check_quantized(c[at], s[at], *swiglu64(rows_value(codes, bits)[perm[at] // K], gate, up, e))
+    dd = own.weight(down.tensor())
+    codes, bits = random_rows(rng, P, n_in)
+    x, v = own.rows8(P, n_in, codes, bits), rows_value(codes, bits)
+    to = np.zeros(P, bool)
+    to[perm[written]] = True
+    for y_type in (F32, BF16):
+        y = own.zeros(P * out // (2 if y_type == BF16 else 1), 0x55555555)
+        with gpu.batch() as b:
+            b.expert_matmul_q8(dd, x, ob, pb, y, y_type)
+        raw = gpu.read_u32(y).view(np.uint8).reshape(P, -1)
+        assert np.all(raw[~to] == 0x55) and not np.any((raw[to] == 0x55).all(1))
+        got = (gpu.read(y) if y_type == F32 else read_bf16(gpu, y)).reshape(P, out)
+        for e in range(E):
+            at = np.flatnonzero(sure & (expert == e))
+            if at.size:
+                check_rows(got[perm[at]], *product(v[at], down.value(e)), n_in, y_type == BF16)
+
+
+@pytest.mark.parametrize("T,y_type", [(200, F32), (5200, F32), (200, BF16), (2600, BF16)])
+@pytest.mark.parametrize("n_in", [256, 272])
+def test_every_code_in_every_form(gpu, own, T, y_type, n_in):
+    """As above, in tiles too and with a last block that is not whole."""
+    out = 256
+    w = Weight8(np.random.default_rng(11), 1, out, n_in)
+    w.codes[0, :, :] = (np.arange(out)[:, None] + np.arange(n_in)[None, :]) % 256
+    nan = np.zeros(out, bool)
+    nan[[3, 130, 255]] = True                                # NaN in these rows only
+    w.codes[0, ~nan] = np.where((w.codes[0, ~nan] & 0x7F) == 0x7F, 0x30, w.codes[0, ~nan])
+    w.scales[:], w.bits[:] = 1, 1
+    wd = own.weight(w.tensor(dense=True))
+    cols = (np.arange(T) * 37) % n_in
+    codes = np.zeros((T, n_in), np.uint8)
+    codes[np.arange(T), cols] = encode(1.0)
+    bad = np.array([5, T - 2])
+    codes[bad, [n_in - 1, 7]] = [0x7F, 0xFF]                 # NaN in two rows of x
+    x = own.rows8(T, n_in, codes, np.full((T, nblocks(n_in)), 0x3F80, np.uint16))
+    y = own.zeros(T * out if y_type == F32 else T * out // 2)
+    with gpu.batch() as b:
+        b.matmul_q8(wd, x, y, y_type)
+    got = (gpu.read(y) if y_type == F32 else read_bf16(gpu, y)).reshape(T, out)
+    fine = np.ones(T, bool)
+    fine[bad] = False
+    assert np.isnan(got[:, nan]).all() and np.isnan(got[bad]).all()
+    assert np.array_equal(got[fine][:, ~nan], decode(w.codes[0])[:, cols].T[fine][:, ~nan])
+
+
+@pytest.mark.parametrize("T,y_type", [(20, BF16), (5200, F32), (2600, BF16)])
+def test_wide_scales_in_every_form(gpu, own, T, y_type):
+    """Scales over 60 and 80 powers of two; NaN and infinite scales of a row and of
+    a weight block, which reach their own outputs only."""
+    rng = np.random.default_rng(T)
+    n_in, out = 528, 384
+    w = Weight8(rng, 1, out, n_in)
+    w.bits[:] = (2.0 ** rng.integers(-60, 0, w.bits.shape)).astype(np.float32)
+    w.bits[0, 1, 4], w.bits[0, 2, 0] = np.nan, np.inf
+    w.scales[:] = w.bits
+    codes, _ = random_rows(rng, T, n_in)
+    bits = f32_to_bf16_bits((2.0 ** rng.integers(-40, 40, (T, 5))).astype(np.float32)).reshape(T, 5)
+    bits[3, 1], bits[T - 1, 4] = 0x7FC0, 0x7F80
+    wd, x = own.weight(w.tensor(dense=True)), own.rows8(T, n_in, codes, bits)
+    y = own.zeros(T * out if y_type == F32 else T * out // 2)
+    with gpu.batch() as b:
+        b.matmul_q8(wd, x, y, y_type)
+    got = (gpu.read(y) if y_type == F32 else read_bf16(gpu, y)).reshape(T, out).astype(np.float64)
+    assert np.isnan(got[3]).all() and not np.isfinite(got[T - 1]).any()
+    assert np.isnan(got[:, 128:256]).all() and not np.isfinite(got[:, 256:]).any()
+    keep = [t for t in range(T) if t not in (3, T - 1)]
+    with np.errstate(invalid="ignore"):
+        values = w.value()[:128]
+    check_rows(got[keep, :128], *product(rows_value(codes, bits)[keep], values), n_in, y_type == BF16)
+
+
+@pytest.mark.parametrize("P", [30, 3000])
+def test_swiglu_of_rows_that_are_not_finite(gpu, own, P):
+    """A NaN code, a NaN and an infinite scale of a row, a NaN scale of a gate
+    block: what they reach reads back as NaN, what they do not is whole."""
+    rng = np.random.default_rng(P)
+    n_in, ff = 272, 272
+    gate, up = Weight8(rng, 1, ff, n_in), Weight8(rng, 1, ff, n_in)
+    gate.bits[0, 1, 2] = np.nan
+    gate.scales[:] = gate.bits
+    codes, bits = random_rows(rng, P, n_in)
+    bad = [4, 9, P - 1]
+    codes[4, 271], bits[9, 1], bits[P - 1, 0] = 0x7F, 0x7FC0, 0x7F80
+    gd, ud, x, q, ob = own.weight(gate.tensor()), own.weight(up.tensor()), own.rows8(P, n_in, codes, bits), own.rows8(P, ff), own.u32([0, P])
+    with gpu.batch() as b:
+        b.expert_swiglu_q8(gd, ud, x, ob, None, 1, q)
+    c, s = gpu.read_rows8(q)
+    v = rows_value(c, s)
+    assert np.isnan(v[bad]).all() and np.isnan(v[:, 128:256]).all()
+    keep = np.setdiff1d(np.arange(P), bad)
+    with np.errstate(invalid="ignore"):
+        want, dw = swiglu64(rows_value(codes, bits)[keep], gate, up, 0)
+    for cols, blocks in ((slice(0, 128), slice(0, 1)), (slice(256, 272), slice(2, 3))):
+        check_quantized(c[keep, cols], s[keep, blocks], want[:, cols], dw[:, cols])
+
+
+@pytest.mark.parametrize("y_type", [F32, BF16])
+def test_tiles_of_operands_just_under_four_gib(gpu, own, y_type):
+    """Tiles address a matrix by 32-bit offsets: the last rows of 2^32 - 2^14
+    codes of x, then of W."""
+    rng = np.random.default_rng(14)
+    n_in, many, few = 16384, (1 << 18) - 1, 96
+    tail, tb = random_rows(rng, few, n_in)
+    w = Weight8(rng, 1, 64, n_in)
+    x = own.rows8(many, n_in)
+    for b, a in zip(x.buffers, (tail, tb)):
+        raw = a.reshape(-1).view(np.float32)
+        gpu.write(b.view(len(b) - raw.size, raw.size), raw)
+    wd, y = own.weight(w.tensor(dense=True)), own.zeros(many * 64 // (1 if y_type == F32 else 2), 0x55555555)
+    with gpu.batch() as b:
+        b.matmul_q8(wd, x, y, y_type)
+    got = (gpu.read(y) if y_type == F32 else read_bf16(gpu, y)).reshape(many, 64)
+    check_rows(got[-few:], *product(rows_value(tail, tb), w.value()), n_in, y_type == BF16)
+    assert not got[:-few].any()
+    # W: the rows of x of the same buffer, a scale of one for all
+    t = Weight8(rng, 1, 1, 16).tensor(dense=True)
+    t.dims = [n_in, many]
+    wd = own.weight(t)
+    scales = own.upload(np.ones(nblocks(many) * nblocks(n_in), np.float32))
+    wd.c.data, wd.c.scales = x.c.codes, MoeRegionC(scales.ptr, 4 * len(scales))
+    codes, bits = random_rows(rng, 40, n_in)
+    rows, z = own.rows8(40, n_in, codes, bits), own.zeros(40 * many // (1 if y_type == F32 else 2), 0x55555555)
+    with gpu.batch() as b:
+        b.matmul_q8(wd, rows, z, y_type)
+    got = (gpu.read(z) if y_type == F32 else read_bf16(gpu, z)).reshape(40, many)
+    check_rows(got[:, -few:], *product(rows_value(codes, bits), decode(tail)), n_in, y_type == BF16)
+    assert not got[:, :-few].any()
+
+
 @pytest.mark.parametrize("T,n_in,out", [(2600, 16, 64), (2561, 1040, 130), (900, 2064, 770), (300, 256, 2500),
                                         (40, 128, 22000)])
 @pytest.mark.parametrize("y_type", [F32, BF16])
