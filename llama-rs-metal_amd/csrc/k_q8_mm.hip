@@ -515,7 +515,7 @@ __global__ __launch_bounds__(64 * NW, WPS) void stream_kernel(Args a) {
 typedef __attribute__((address_space(3))) void *lds_ptr;
 constexpr uint64_t kCus = 256;
 constexpr uint32_t kStage = 128 * 128;  // bytes of a stage's token rows, half of its weight rows'
-constexpr int kScaleSlots = 32, kGroup = 8, kStages = 3, kTileWaves = 8, kTileRows = 128, kTileCols = 256, kSlots = 8;
+constexpr int kScaleSlots = 32, kGroup = 8, kStages = 3, kTileWaves = 8, kTileRows = 128, kSlots = 8;
 
 struct TileLds {
     uint8_t x[kStages * kStage];
@@ -971,8 +971,8 @@ static hipError_t launch_q8(Prof *p, hipStream_t s, const char *name, q8::Args a
     // SwiGLU's steps are worth it from the first row on (2048 to 512, 512 experts: 640 rows 132, 144).
     // DMA offsets and the scales' indexes there are 32-bit.
     constexpr uint64_t kRows = MODE == SWIGLU ? 0 : MODE == F32OUT ? 16 : 12;
-    const bool fills = ct * a.P >= (MODE == F32OUT ? 5120 : 2560) || (MODE == BF16OUT && ct * live >= 80) ||
-                       (MODE == SWIGLU && ct * (a.P + 32 * live) >= 3520);
+    const bool fills = ct * a.P >= (MODE == F32OUT ? 2 * kQ8FewRows : kQ8FewRows) || (MODE == BF16OUT && ct * live >= 80) ||
+                       (MODE == SWIGLU && ct * (a.P + 32 * live) >= kQ8FewWork);
     const bool tiled = fills && a.P >= kRows * experts && (uint64_t)a.xrows * a.in < 0xffffffffull &&
                        (uint64_t)a.out * a.in < 0xffffffffull &&
                        (uint64_t)experts * ((a.out + 127) / 128) * a.kb < 0xffffffffull;

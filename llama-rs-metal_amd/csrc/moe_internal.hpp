@@ -284,10 +284,14 @@ hipError_t launch_q8_rows(Prof *p, hipStream_t s, const char *name, const Q8Weig
                           const uint32_t *offsets, const uint32_t *perm, void *y, bool bf16);
 // out[p] = silu(x_t . G_e) * (x_t . U_e), t = perm[p] / k (perm null: p);
 // rows: an engine's kQ8SpaceLen words, for few positions: F32 rows of kQ8RowsLen
-// values and a list of kQ8TilesLen tiles (with fewer than 2560 positions times
-// blocks of 128 outputs, and 3520 with 32 more positions for each segment, there
-// are at most P / 16 + (3520 - P) / 32 < 190 tiles)
-constexpr uint64_t kQ8RowsLen = 2560 * 128, kQ8TilesLen = 256, kQ8SpaceLen = kQ8RowsLen + 2 + 2 * kQ8TilesLen;
+// values and a list of kQ8TilesLen tiles.
+// Few are P positions in S segments over B blocks of 128 outputs with
+// B * P < kQ8FewRows and B * (P + 32 * S) < kQ8FewWork (measured at the rule that uses
+// them): fewer than kQ8FewRows * 128 values, and P / 16 + S tiles of 16 rows at
+// most, which are fewer than P / 32 + kQ8FewWork / 32.
+constexpr uint64_t kQ8FewRows = 2560, kQ8FewWork = 3520;
+constexpr uint64_t kQ8RowsLen = kQ8FewRows * 128, kQ8TilesLen = (kQ8FewRows + kQ8FewWork) / 32;
+constexpr uint64_t kQ8SpaceLen = kQ8RowsLen + 2 + 2 * kQ8TilesLen;
 hipError_t launch_q8_swiglu(Prof *p, hipStream_t s, const Q8Weight &gate, const Q8Weight &up, const Q8Rows &x,
                             const uint32_t *offsets, const uint32_t *perm, uint32_t k, const Q8Rows &out,
                             float *rows);

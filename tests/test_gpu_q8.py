@@ -782,6 +782,28 @@ def test_small_swiglu_after_more_tiles_than_a_launch_has(gpu, own, T, n_in, ff, 
             assert np.array_equal(i, j)
 
 
+@pytest.mark.parametrize("P,E,ff", [(2559, 1, 128), (1279, 1, 256), (2000, 47, 128), (2400, 34, 16), (106, 106, 16), (900, 26, 256)])
+def test_the_largest_swiglus_in_two_launches(gpu, own, P, E, ff):
+    """As many rows, and tiles, as the F32 rows and the list between the launches
+    are for; one more of either goes in tiles of 128."""
+    rng = np.random.default_rng(P)
+    n_in = 144
+    for P, E in ((P, E), (P + 1, E + 1)):
+        w, w2 = Weight8(rng, E, ff, n_in), Weight8(rng, E, ff, n_in)
+        offsets, perm = segments(rng, 1 + np.bincount(rng.integers(0, E, P - E), minlength=E))
+        codes, bits = random_rows(rng, P, n_in)
+        wd, ud, x, q = own.weight(w.tensor()), own.weight(w2.tensor()), own.rows8(P, n_in, codes, bits), own.rows8(P, ff)
+        ob, pb = own.u32(offsets), own.u32(perm)
+        with gpu.batch() as b:
+            b.expert_swiglu_q8(wd, ud, x, ob, pb, 1, q)
+        c, s = gpu.read_rows8(q)
+        v = rows_value(codes, bits)[perm]
+        for e in range(E):
+            a, b_ = offsets[e], offsets[e + 1]
+            if b_ > a:
+                check_quantized(c[a:b_], s[a:b_], *swiglu64(v[a:b_], w, w2, e))
+
+
 def test_more_tiles_than_32_bits_count(gpu, own):
     """8192 segments of all rows, 2^32 + 8192 tiles of 128: those of the first
     segments run, and with them every row has its product."""
