@@ -491,11 +491,15 @@ class Gpu:
         nb = rows * n, rows * (-(-n // 128)) * 2
         bufs = [self.zeros(-(-b // 4)) for b in nb]
         r = Rows8(MoeRegionC(bufs[0].c.ptr, nb[0]), MoeRegionC(bufs[1].c.ptr, nb[1]), rows, n, bufs)
-        if codes is not None:
+        if codes is not None or scales is not None:
             self.write_rows8(r, codes, scales)
         return r
 
     def write_rows8(self, r, codes, scales):
+        if not r.buffers:
+            raise ShapeError("8-bit rows without buffers of their own")
+        if codes is None or scales is None or np.size(codes) != r.rows * r.n or np.size(scales) != r.rows * (-(-r.n // 128)):
+            raise ShapeError("8-bit rows: code/scale length")
         for b, a, dt in zip(r.buffers, (codes, scales), (np.uint8, np.uint16)):
             raw = np.zeros(4 * len(b), np.uint8)
             a = np.ascontiguousarray(a, dt).ravel().view(np.uint8)
@@ -504,6 +508,8 @@ class Gpu:
 
     def read_rows8(self, r):
         """(codes uint8 [rows, n], bf16 scale bits uint16 [rows, ceil(n/128)])"""
+        if not r.buffers:
+            raise ShapeError("8-bit rows without buffers of their own")
         c, s = (self.read(b).view(np.uint8) for b in r.buffers)
         nb = -(-r.n // 128)
         return c[:r.rows * r.n].reshape(r.rows, r.n), s.view(np.uint16)[:r.rows * nb].reshape(r.rows, nb)

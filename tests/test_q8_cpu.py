@@ -2,9 +2,10 @@
 import ctypes as C
 
 import numpy as np
+import pytest
 
 from helpers_q8 import POS, TABLE, Weight8, decode, encode, nblocks, quantize_rows, random_rows, rows_value
-from hip_backend import BF16, E4M3, F16, F32, api
+from hip_backend import BF16, E4M3, F16, F32, Buffer, Gpu, Rows8, ShapeError, api
 
 
 def test_e4m3_codes_round_to_nearest_even():
@@ -56,3 +57,39 @@ def test_block8_tensors_hold_codes_and_block_scales():
         assert w.value(2).shape == (130, 272) and nblocks(272) == 3
     codes, bits = random_rows(rng, 4, 48)
     assert codes.shape == (4, 48) and bits.shape == (4, 1)
+
+
+class Memory:
+    """Takes a Gpu's writes on the host."""
+
+    write_rows8 = Gpu.write_rows8
+
+    def __init__(self):
+        self.written = []
+
+    def zeros(self, n):
+        return Buffer(None, api.MoeBufferC(0x1000, n), 0x1000)
+
+    def write(self, b, a):
+        self.written.append(a.view(np.uint8))
+
+
+def test_rows8_are_written_whole_or_refused():
+    rows, n = 3, 272
+    codes, bits = np.ones((rows, n), np.uint8), np.ones((rows, 3), np.uint16)
+    m = Memory()
+    r = Gpu.rows8(m, rows, n)
+    for c, s in ((codes[:2], bits), (codes, bits[:2]), (codes, bits[:, :2]), (codes[:, :-16], bits), (codes, None),
+                 (None, bits), (np.ones((rows + 1, n), np.uint8), bits), (codes, np.ones((rows, 4), np.uint16))):
+        with pytest.raises(ShapeError):
+            Gpu.write_rows8(m, r, c, s)
+        with pytest.raises(ShapeError):
+            Gpu.rows8(m, rows, n, c, s)
+    own = Rows8(api.MoeRegionC(), api.MoeRegionC(), rows, n)      # regions that the caller holds
+    with pytest.raises(ShapeError):
+        Gpu.write_rows8(m, own, codes, bits)
+    with pytest.raises(ShapeError):
+        Gpu.read_rows8(m, own)
+    assert not m.written
+    Gpu.write_rows8(m, r, codes, bits)
+    assert [a.size for a in m.written] == [816, 20] and m.written[0].all() and m.written[1][:18:2].all()
