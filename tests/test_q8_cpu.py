@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 from helpers_q8 import POS, TABLE, Weight8, decode, encode, nblocks, quantize_rows, random_rows, rows_value
-from hip_backend import BF16, E4M3, F16, F32, Buffer, Gpu, Rows8, ShapeError, api
+from hip_backend import BF16, E4M3, F16, F32, Buffer, Gpu, Rows8, ShapeError, Weight, api
 
 
 def test_e4m3_codes_round_to_nearest_even():
@@ -93,3 +93,21 @@ def test_rows8_are_written_whole_or_refused():
     assert not m.written
     Gpu.write_rows8(m, r, codes, bits)
     assert [a.size for a in m.written] == [816, 20] and m.written[0].all() and m.written[1][:18:2].all()
+
+
+def test_reshaped_weights_keep_the_blocks_of_their_scales():
+    def weight(dims, dtype=E4M3):
+        c = api.MoeWeightC()
+        c.dtype, c.ndims = dtype, len(dims)
+        c.dims[:len(dims)] = dims
+        return Weight(c, [], dims, 0)
+
+    for dims, to in (([272, 130], [272, 130, 1]), ([272, 130, 1], [272, 130]), ([272, 256, 3], [272, 768]),
+                     ([272, 768], [272, 256, 3]), ([272, 256, 3], [272, 384, 2])):
+        r = weight(dims).reshape(to)
+        assert r.dims == to and list(r.c.dims[:len(to)]) == to and r.c.ndims == len(to)
+    for dims, to in (([256, 256], [512, 128]), ([272, 130, 4], [272, 520]), ([272, 520], [272, 130, 4]),
+                     ([272, 192, 2], [272, 128, 3]), ([256, 128], [256 * 128]), ([16, 4, 2], [16, 8])):
+        with pytest.raises(ShapeError):
+            weight(dims).reshape(to)
+        assert weight(dims, F32).reshape(to).dims == to
