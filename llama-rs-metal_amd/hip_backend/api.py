@@ -290,7 +290,7 @@ class Weight:
             raise ShapeError("weight reshape")
         if self.bits and dims[0] != self.dims[0]:
             raise ShapeError("affine reshape must preserve row width")
-        if self.c.dtype == E4M3 and (len(dims) < 2 or dims[0] != self.dims[0] or
+        if self.c.dtype == E4M3 and (min(len(dims), len(self.dims)) < 2 or dims[0] != self.dims[0] or
                                      (dims[1] != self.dims[1] and (dims[1] % 128 or self.dims[1] % 128))):
             raise ShapeError("8-bit reshape must preserve the 128 x 128 blocks of the scales")
         c = MoeWeightC.from_buffer_copy(self.c)
