@@ -324,12 +324,15 @@ moe_status moe_block_noalloc(moe_gpu *gpu, const moe_block_weights *w, moe_buffe
  * [E][out][in], group_size 128, `scales` one scale_type value (F32, F16 or
  * BF16) per block, [E][ceil(out/128)][ceil(in/128)], biases unused; a value is
  * code * scale.  dims[0] is a multiple of 16 and the codes start 16-byte
- * aligned.
+ * aligned.  in <= 2^24, out < 2^31, E <= 16384, rows < 2^31; a launch of
+ * more threads than 2^32 (2^36 outputs and more) is an error and leaves y as it was.
  *
  * Products multiply the codes exactly.  F32 outputs are F32 sums.  Outputs in
  * BF16 or 8 bits use matrix instructions on the codes themselves, which align
  * eight products at a time to the largest of them and cut each at 2^-13 of its
- * power of two; sums of eight, blocks and scales join in F32. */
+ * power of two; sums of eight, blocks and scales join in F32.  A block's two scales
+ * are multiplied first: a product of scales below 2^-126 has lost digits, one
+ * past F32's range is infinite. */
 
 /* Rows in 8 bits: codes [rows, n], n a multiple of 16, 16-byte aligned, and one
  * BF16 scale per row and 128 columns, [rows, ceil(n/128)].  Quantised here:
@@ -355,10 +358,12 @@ moe_status moe_matmul_q8(moe_gpu *gpu, const moe_weight *w, moe_rows8 x, moe_buf
                          uint32_t y_type);
 /* Grouped by expert, over segments as moe_dispatch writes them: position p of
  * [offsets[e], offsets[e+1]) belongs to expert e, and perm[p] is its pair
- * t*k + i.  q[p] = silu(x_t . G_e) * (x_t . U_e) in 8 bits, in position order;
- * q.rows = x.rows * k positions.  perm empty: position p reads row p (k = 1).
+ * t*k + i.  q[p] = silu(x_t . G_e) * (x_t . U_e) in 8 bits (silu's exponential
+ * within 2^-16), in position order; q.rows = x.rows * k positions.  perm empty:
+ * position p reads row p (k = 1).  gate and up have the same dims and scale_type.
  * Ends past q.rows count as q.rows; positions of no segment, and positions
- * whose perm names no row, are left as they were.  Segments do not overlap. */
+ * whose perm names no row, are left as they were.  Segments do not overlap: a
+ * position of two is of either, or left as it was. */
 moe_status moe_expert_swiglu_q8(moe_gpu *gpu, const moe_weight *gate, const moe_weight *up,
                                 moe_rows8 x, moe_buffer offsets, moe_buffer perm, uint64_t k,
                                 moe_rows8 q);
@@ -369,7 +374,7 @@ moe_status moe_expert_matmul_q8(moe_gpu *gpu, const moe_weight *w, moe_rows8 x,
                                 moe_buffer offsets, moe_buffer perm, moe_buffer y, uint32_t y_type);
 /* moe_mix for every token: y[t] = sum_i w[t*k + i] * x[t*k + i] (i ascending)
  * (+ residual[t], which may be exactly y); w holds tokens * k values, x F32 or
- * bf16 rows of y.len / tokens values. */
+ * bf16 (two per element; an even number of values) rows of y.len / tokens values. */
 moe_status moe_mix_tokens(moe_gpu *gpu, moe_buffer x, uint32_t x_type, moe_buffer w,
                           moe_buffer residual, moe_buffer y, uint64_t tokens);
 
