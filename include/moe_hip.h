@@ -362,8 +362,8 @@ moe_status moe_matmul_q8(moe_gpu *gpu, const moe_weight *w, moe_rows8 x, moe_buf
  * within 2^-16), in position order; q.rows = x.rows * k positions.  perm empty:
  * position p reads row p (k = 1).  gate and up have the same dims and scale_type.
  * Ends past q.rows count as q.rows; positions of no segment, and positions
- * whose perm names no row, are left as they were.  Segments do not overlap: a
- * position of two is of either, or left as it was. */
+ * whose perm names no row, are left as they were.  Segments do not overlap: each
+ * value of a position of two is that of either, or left as it was. */
 moe_status moe_expert_swiglu_q8(moe_gpu *gpu, const moe_weight *gate, const moe_weight *up,
                                 moe_rows8 x, moe_buffer offsets, moe_buffer perm, uint64_t k,
                                 moe_rows8 q);
