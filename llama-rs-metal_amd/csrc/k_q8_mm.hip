@@ -960,15 +960,16 @@ static hipError_t launch_q8(Prof *p, hipStream_t s, const char *name, q8::Args a
     auto max_tiles = [&](uint32_t bm) { return a.P / bm + (a.offsets ? live : (uint64_t)(a.P % bm != 0)); };
     // Tiles of 128 rows need CUs to work on them: enough items, or enough rows
     // (2048 columns, microseconds of tiles against the best stream form):
-    //   SwiGLU  512 outputs, 1 expert, 512 rows (16 items): 19.1, 15.4;  4 experts, 1024 rows (32): 19.9, 46.3
-    //           768 outputs, 16 experts, 16 rows (96 items): 15.2, 11.2;  128 rows: 15.6, 16.6;  256 rows: 15.5, 20.5
-    //           512 outputs, 512 experts, 20 rows (80 items): 15.5, 14.6;  40 rows (160): 18.7, 22.9
+    //   SwiGLU  512 outputs, 1 expert, 512 rows (16 items): 19.1, 15.4;  4 experts, 1024 rows (32): 19.7, 45.9
+    //           768 outputs, 16 experts, 16 rows (96 items): 15.3, 12.5;  128 rows: 15.6, 17.8;  256 rows: 15.7, 28.0
+    //           512 outputs, 512 experts, 20 rows (80 items): 15.7, 16.2;  40 rows (160): 19.6, 24.7
     //   bf16    4096 outputs, 128 rows (16 items): 16.0, 13.2;  256 rows (32): 16.4, 19.1
     //           16384 outputs, 32 rows (64 items): 13.7, 13.6;  48 rows: 13.8, 19.4
     //   F32     4096 outputs, 256 rows (32 items): 31.5, 20.3;  512 rows (64): 33.5, 38.3
     // and an expert's rows to be worth its steps (768 columns to 2048, 64 experts):
     //   bf16    512 rows: 21.3, 18.7;  1024: 21.7, 24.9      F32  512 rows: 23.5, 19.6;  1024: 24.1, 26.1
-    // SwiGLU's steps are worth it from the first row on (2048 to 512, 512 experts: 640 rows 132, 144).
+    // SwiGLU's steps are worth it from the first row on (2048 to 512, 64 experts, 64 rows: 20.4, 24.7;
+    // 512 experts, 640 rows: 131, 129).
     // DMA offsets and the scales' indexes there are 32-bit.
     constexpr uint64_t kRows = MODE == SWIGLU ? 0 : MODE == F32OUT ? 16 : 12;
     const bool fills = ct * a.P >= (MODE == F32OUT ? 2 * kQ8FewRows : kQ8FewRows) || (MODE == BF16OUT && ct * live >= 80) ||
@@ -986,7 +987,7 @@ static hipError_t launch_q8(Prof *p, hipStream_t s, const char *name, q8::Args a
     if constexpr (MODE == SWIGLU) {
         // A scale needs 128 outputs: blocks that hold them (512 KiB of weights at
         // 2048 columns) are few, so blocks of 16 to 64 write F32 rows and a second
-        // launch quantises them (10 rows of 512 experts: 20.2 us, 12.3).  One launch
+        // launch quantises them (10 rows of 512 experts: 20.2 us, 12.1).  One launch
         // whose last block of each 128 quantises took 11.1 where the rows' order
         // rested on their stores having landed; 14.2 with a release and an acquire
         // around the count, which write back and drop a whole L2.  (What does not
