@@ -324,8 +324,9 @@ moe_status moe_block_noalloc(moe_gpu *gpu, const moe_block_weights *w, moe_buffe
  * [E][out][in], group_size 128, `scales` one scale_type value (F32, F16 or
  * BF16) per block, [E][ceil(out/128)][ceil(in/128)], biases unused; a value is
  * code * scale.  dims[0] is a multiple of 16 and the codes start 16-byte
- * aligned.  in <= 2^24, out < 2^31, E <= 16384, rows < 2^31; a launch of
- * more threads than 2^32 (2^36 outputs and more) is an error and leaves y as it was.
+ * aligned.  in <= 2^24, out < 2^31, E <= 16384, rows < 2^31; a call that takes
+ * 2^32 threads or more is an error and leaves its outputs as they were (an
+ * expert's 16 rows of 128 outputs take 256, in SwiGLU 512).
  *
  * Products multiply the codes exactly.  F32 outputs are F32 sums.  Outputs in
  * BF16 or 8 bits use matrix instructions on the codes themselves, which align

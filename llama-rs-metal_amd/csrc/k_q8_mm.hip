@@ -946,7 +946,7 @@ static hipError_t launch_form(Prof *p, hipStream_t s, const char *name, const Fo
     uint64_t blocks = (tiles * a.col_tiles + q8::kXcds - 1) / q8::kXcds * q8::kXcds;
     if (blocks > 0x7ffffff8ull) return hipErrorInvalidConfiguration;
     if (blocks > most_blocks) blocks = most_blocks;
-    if (blocks * f.threads > 0xffffffffull) return hipErrorInvalidConfiguration;  // (outputs of more than 2^36 values)
+    if (blocks * f.threads > 0xffffffffull) return hipErrorInvalidConfiguration;  // (2^34 outputs or more, or tiles of few rows)
     return launch_kernel(p, name, f.kernel, dim3((uint32_t)blocks), dim3(f.threads), 0, s, a);
 }
 
