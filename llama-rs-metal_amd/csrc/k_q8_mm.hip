@@ -972,7 +972,7 @@ static hipError_t launch_q8(Prof *p, hipStream_t s, const char *name, q8::Args a
     // 512 experts, 640 rows: 131, 129).
     // DMA offsets and the scales' indexes there are 32-bit.
     constexpr uint64_t kRows = MODE == SWIGLU ? 0 : MODE == F32OUT ? 16 : 12;
-    const bool fills = ct * a.P >= (MODE == F32OUT ? 2 * kQ8FewRows : kQ8FewRows) || (MODE == BF16OUT && ct * live >= 80) ||
+    const bool fills = ct * a.P >= (MODE == SWIGLU ? kQ8FewRows : MODE == F32OUT ? 5120 : 2560) || (MODE == BF16OUT && ct * live >= 80) ||
                        (MODE == SWIGLU && ct * (a.P + 32 * live) >= kQ8FewWork);
     const bool tiled = fills && a.P >= kRows * experts && (uint64_t)a.xrows * a.in < 0xffffffffull &&
                        (uint64_t)a.out * a.in < 0xffffffffull &&
