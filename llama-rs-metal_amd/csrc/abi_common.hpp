@@ -103,14 +103,13 @@ struct Range {
     uintptr_t lo, hi;  // [lo, hi)
     bool empty() const { return hi <= lo; }
 };
-inline Range rng(const moe_buffer &b) {
-    uintptr_t p = reinterpret_cast<uintptr_t>(b.ptr);
-    return Range{p, p + b.len * 4};
+// (a length that does not fit the address space ends at its end, in no allocation)
+inline Range span(const void *ptr, uint64_t n, uint64_t size) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(ptr);
+    return Range{p, n > (UINTPTR_MAX - p) / size ? UINTPTR_MAX : p + n * size};
 }
-inline Range rng(const moe_region &r) {
-    uintptr_t p = reinterpret_cast<uintptr_t>(r.ptr);
-    return Range{p, p + r.bytes};
-}
+inline Range rng(const moe_buffer &b) { return span(b.ptr, b.len, 4); }
+inline Range rng(const moe_region &r) { return span(r.ptr, r.bytes, 1); }
 inline bool overlaps(const Range &a, const Range &b) {
     return !a.empty() && !b.empty() && a.lo < b.hi && b.lo < a.hi;
 }

@@ -1021,6 +1021,20 @@ def test_refusals(gpu, own):
         b.matmul_q8(w2, x, y)
 
 
+def test_lengths_past_the_address_space_are_refused(gpu, own):
+    """2^62 + 4 elements are 16 bytes in 64 bits: not those of an allocation."""
+    a, b_ = own.zeros(64), own.zeros(64)
+    for n in ((1 << 62) + 4, (1 << 63) + 4, (1 << 64) - 8):
+        long, other = (Buffer(gpu, MoeBufferC(x.ptr + 32, n), x.ptr) for x in (a, b_))
+        with pytest.raises(ShapeError):
+            gpu.clear(long)
+        with gpu.batch() as b:
+            for f in (lambda: b.copy(long, other), lambda: b.add(long, other, long),
+                      lambda: b.mix_tokens(long, long, None, other, n)):
+                with pytest.raises(ShapeError):
+                    f()
+
+
 # ------------------------------------------------------------------ chain --
 def chain(b, o, d):
     """One MoE block over T tokens by the operators."""
